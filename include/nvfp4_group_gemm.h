@@ -33,7 +33,10 @@ extern "C" {
 /* 2: segment launches (nvfp4_grouped_gemm_segments, nvfp4_segment_output), the
  * expert-parallel exchange (nvfp4_ep_*), NVFP4_FLAG_SPLIT_K, a segment-row table in the
  * workspace (nvfp4_workspace_size grew by 4 bytes per group, rounded up to 128). */
-#define NVFP4_ABI_VERSION 2
+/* 3: int8 products (nvfp4_int8_gemm, nvfp4_quantize_int8, nvfp4_moe_dispatch_int8), token sort
+ * with gradients (nvfp4_moe_dispatch_tokens, nvfp4_moe_combine_tokens and its backward),
+ * NVFP4_DTYPE_FP32. */
+#define NVFP4_ABI_VERSION 3
 
 typedef enum nvfp4_status {
   NVFP4_OK = 0,
@@ -230,6 +233,7 @@ NVFP4_API int nvfp4_sf_to_blocked(const void* plain, void* blocked, int rows, in
  */
 #define NVFP4_DTYPE_BF16 0
 #define NVFP4_DTYPE_FP16 1
+#define NVFP4_DTYPE_FP32 2 /* token sort and int8 product outputs; the quantisers take 0 and 1 */
 NVFP4_API int nvfp4_quantize(const void* x, int rows, int cols, int64_t ld, int dtype,
                              float global_scale, void* packed, int64_t packed_ld, void* sf_blocked,
                              void* stream);
@@ -293,6 +297,99 @@ NVFP4_API int nvfp4_moe_gather_quantized(const void* packed_src, int64_t ld_src,
 NVFP4_API int nvfp4_moe_combine(const void* y, int64_t ldy, const int32_t* dest,
                                 const float* weights, int tokens, int topk, int cols, void* out,
                                 int64_t ldo, void* stream);
+
+/*
+ * Tokens sorted by expert and back, with gradients (no counterpart in the reference, which is
+ * inference only). dtype is NVFP4_DTYPE_BF16, _FP16 or _FP32 for every row argument; dest
+ * [tokens * topk] and src_rows [rows] are nvfp4_moe_route's (pairs whose row is outside
+ * [0, rows) are dropped pairs; every other row may be named by one pair only). Any column
+ * count, alignment and row stride; rows on 16-byte boundaries move fastest.
+ *   dispatch: y[dest[t, j]] = x[t]; zeros on the rows with src_rows[r] < 0
+ *   combine:  out[t] = sum_j weights[t, j] * y[dest[t, j]] (fp32 products and sums in slot
+ *             order, rounded once; weights NULL: ones). Without weights this is the gradient
+ *             of dispatch with respect to x.
+ *   combine_backward: grad_y[dest[t, j]] = weights[t, j] * grad_out[t], zeros on rows with
+ *             src_rows[r] < 0; grad_w[t, j] = <grad_out[t], y[dest[t, j]]> in fp32, 0 for
+ *             dropped pairs. Either gradient may be NULL (not wanted).
+ */
+NVFP4_API int nvfp4_moe_dispatch_tokens(const void* x, int64_t ldx, int dtype, const int32_t* dest,
+                                        const int32_t* src_rows, int tokens, int topk, int cols,
+                                        int64_t rows, void* y, int64_t ldy, void* stream);
+NVFP4_API int nvfp4_moe_combine_tokens(const void* y, int64_t ldy, int dtype, const int32_t* dest,
+                                       const float* weights, int tokens, int topk, int cols,
+                                       int64_t rows, void* out, int64_t ldo, void* stream);
+NVFP4_API int nvfp4_moe_combine_tokens_backward(const void* grad_out, int64_t ldg, const void* y,
+                                                int64_t ldy, int dtype, const int32_t* dest,
+                                                const int32_t* src_rows, const float* weights,
+                                                int tokens, int topk, int cols, int64_t rows,
+                                                void* grad_y, int64_t ldo, float* grad_w,
+                                                void* stream);
+
+/*
+ * int8 row quantiser (no counterpart in the reference): scales[r] = max_k |x[r, k]| / 127,
+ * codes[r, k] = 127 * x[r, k] / max|x[r]| rounded to nearest, ties to even, of the exact
+ * quotient. x bf16 or fp16 [rows, cols], any alignment and row stride ld (elements); codes
+ * int8, 16-byte aligned, row stride codes_ld a multiple of 16 bytes (bytes past cols are not
+ * written). A row of zeros has scale 0; a row holding an infinity or a NaN has scale NaN and
+ * zero codes. row_mask (or NULL): rows with row_mask[r] < 0 are neither read nor written.
+ * nvfp4_moe_dispatch_int8 quantises each token once and writes its codes and scale to the
+ * rows dest[t * topk + j] inside [0, rows); other rows are not written.
+ */
+NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
+                                  const int32_t* row_mask, void* codes, int64_t codes_ld,
+                                  float* scales, void* stream);
+NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
+                                      const int32_t* dest, int topk, int64_t rows, void* codes,
+                                      int64_t codes_ld, float* scales, void* stream);
+
+/*
+ * int8 matrix product with a scale per token and per channel (no counterpart in the
+ * reference). For every row t of expert e's segment
+ *   out[t, n] = a_scale[t] * b_scale[e, n] * sum_k a[t, k] * b[e, n, k] (+ bias[n])
+ * or, with b2 and b2_scale, silu(that with b) * (that with b2), fp32 until one rounding to
+ * out_dtype (NVFP4_DTYPE_*). The sums are exact (int32; k <= 131071).
+ *
+ * a [rows, k] and b [num_experts * n, k] (and b2) are int8, 16-byte aligned, rows lda / ldb
+ * bytes apart (multiples of 16; k itself may be anything); out has row stride ldo elements and
+ * any alignment. Segments: device int32 seg_offsets / seg_counts [num_experts], or both NULL
+ * with one expert (the whole of a). They may start at any row; rows outside every segment are
+ * left as they were; a segment outside [0, rows) is skipped and reported by nvfp4_int8_check.
+ * expected_rows (0: rows) is the host's estimate of the rows in all segments; it picks the
+ * tile shape only. bias needs one expert and no b2. num_experts <= 1024.
+ *
+ * Needs no workspace and keeps nothing between calls: calls may overlap on any streams and in
+ * any CUDA graphs.
+ */
+typedef struct nvfp4_int8_product {
+  const void* a;
+  const void* b;
+  const void* b2;
+  const float* a_scale;
+  const float* b_scale;
+  const float* b2_scale;
+  const float* bias;
+  void* out;
+  const int32_t* seg_offsets;
+  const int32_t* seg_counts;
+  int64_t rows;
+  int64_t lda;
+  int64_t ldb;
+  int64_t ldo;
+  int64_t expected_rows;
+  int32_t n;
+  int32_t k;
+  int32_t num_experts;
+  int32_t out_dtype;
+} nvfp4_int8_product;
+
+NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* product, void* stream);
+
+/*
+ * Synchronise `stream`, then read and clear the current device's error word of the int8
+ * products: NVFP4_ERR_DEVICE_TIMEOUT when a kernel gave up on a wait, NVFP4_ERR_BAD_SHAPE when
+ * a segment was outside its slab (skipped).
+ */
+NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits);
 
 /*
  * Expert-parallel MoE exchange over NVLink peer memory: one process per GPU, `world` ranks

@@ -79,9 +79,16 @@ EXPORTED_SYMBOLS = (
     "nvfp4_ep_publish_pairs",
     "nvfp4_ep_return_sums",
     "nvfp4_ep_combine_sums",
+    "nvfp4_moe_dispatch_tokens",
+    "nvfp4_moe_combine_tokens",
+    "nvfp4_moe_combine_tokens_backward",
+    "nvfp4_quantize_int8",
+    "nvfp4_moe_dispatch_int8",
+    "nvfp4_int8_gemm",
+    "nvfp4_int8_check",
 )
 
-ABI_VERSION = 2   # NVFP4_ABI_VERSION
+ABI_VERSION = 3   # NVFP4_ABI_VERSION
 EP_MAX_RANKS = 8  # NVFP4_EP_MAX_RANKS
 MAX_REPLICAS = 7  # replicas nvfp4_grouped_gemm_replicated accepts
 EP_ERR_CAPACITY = 1 << 0  # an expert segment did not fit the owner's receive slab
@@ -128,9 +135,14 @@ class EpPeers(ctypes.Structure):
 ROWS_GATHER = 1
 ROWS_MASK = 2
 
-# Input dtypes of nvfp4_quantize (NVFP4_DTYPE_*).
+# Element types (NVFP4_DTYPE_*).
 DTYPE_BF16 = 0
 DTYPE_FP16 = 1
+DTYPE_FP32 = 2
+
+# Limits of nvfp4_int8_gemm.
+INT8_MAX_EXPERTS = 1024
+INT8_MAX_K = 131071
 
 # Largest group count nvfp4_grouped_gemm_noalloc accepts (NVFP4_NOALLOC_MAX_GROUPS).
 NOALLOC_MAX_GROUPS = 512
@@ -158,7 +170,33 @@ class Nvfp4Group(ctypes.Structure):
     ]
 
 
-# The same record as a numpy structured dtype, so that a whole group table is
+class Int8Product(ctypes.Structure):
+    """Mirror of ``nvfp4_int8_product``."""
+
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("b2", ctypes.c_void_p),
+        ("a_scale", ctypes.c_void_p),
+        ("b_scale", ctypes.c_void_p),
+        ("b2_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("seg_offsets", ctypes.c_void_p),
+        ("seg_counts", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("lda", ctypes.c_int64),
+        ("ldb", ctypes.c_int64),
+        ("ldo", ctypes.c_int64),
+        ("expected_rows", ctypes.c_int64),
+        ("n", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("num_experts", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+    ]
+
+
+# Nvfp4Group as a numpy structured dtype, so that a whole group table is
 # filled with a few vectorised column assignments instead of per-field ctypes calls.
 GROUP_DTYPE = np.dtype(
     {
@@ -275,6 +313,24 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.nvfp4_ep_return_sums.restype = i32
         lib.nvfp4_ep_combine_sums.argtypes = [vp, vp, i32, i32, i32, i32, vp, i32, vp, i64, vp]
         lib.nvfp4_ep_combine_sums.restype = i32
+        lib.nvfp4_moe_dispatch_tokens.argtypes = [vp, i64, i32, vp, vp, i32, i32, i32, i64, vp,
+                                                  i64, vp]
+        lib.nvfp4_moe_dispatch_tokens.restype = i32
+        lib.nvfp4_moe_combine_tokens.argtypes = [vp, i64, i32, vp, vp, i32, i32, i32, i64, vp,
+                                                 i64, vp]
+        lib.nvfp4_moe_combine_tokens.restype = i32
+        lib.nvfp4_moe_combine_tokens_backward.argtypes = [vp, i64, vp, i64, i32, vp, vp, vp, i32,
+                                                          i32, i32, i64, vp, i64, vp, vp]
+        lib.nvfp4_moe_combine_tokens_backward.restype = i32
+        lib.nvfp4_quantize_int8.argtypes = [vp, i64, i32, i64, i32, vp, vp, i64, vp, vp]
+        lib.nvfp4_quantize_int8.restype = i32
+        lib.nvfp4_moe_dispatch_int8.argtypes = [vp, i32, i32, i64, i32, vp, i32, i64, vp, i64, vp,
+                                                vp]
+        lib.nvfp4_moe_dispatch_int8.restype = i32
+        lib.nvfp4_int8_gemm.argtypes = [ctypes.POINTER(Int8Product), vp]
+        lib.nvfp4_int8_gemm.restype = i32
+        lib.nvfp4_int8_check.argtypes = [vp, ctypes.POINTER(ctypes.c_uint)]
+        lib.nvfp4_int8_check.restype = i32
         if path is None:
             _lib = lib
         return lib

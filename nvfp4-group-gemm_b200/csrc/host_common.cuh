@@ -1,8 +1,9 @@
 // Host-side helpers shared by the library's translation units: the per-thread error
 // detail of the last failing call, status helpers, and the per-device state (SM count,
-// kernel attributes set once per device).
+// kernel attributes set once per device), tensor-map encoding and kernel launches.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -20,6 +21,33 @@ extern thread_local std::string g_last_error;
 int fail(int code, const char* fmt, ...);
 // NVFP4_ERR_CUDA with the CUDA error's name and text.
 int cuda_fail(cudaError_t e, const char* what);
+
+// cuTensorMapEncodeTiled (resolved through the runtime) without interleave, zero fill outside
+// the tensor. False when the encoder is missing or rejects the map.
+bool encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, unsigned rank, void* addr,
+                      const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                      const cuuint32_t* elem_strides, CUtensorMapSwizzle swizzle,
+                      CUtensorMapL2promotion promotion);
+
+// Launch with programmatic stream serialization: the kernel may be scheduled while its
+// predecessor in the stream drains, and must run griddepcontrol.wait before it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, int smem,
+                             cudaStream_t stream, const Args&... args) {
+  if (grid <= 0) return cudaSuccess;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

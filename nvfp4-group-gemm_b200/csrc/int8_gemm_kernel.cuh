@@ -1,0 +1,353 @@
+// int8 matrix product with a scale per token and per channel, over one or many row segments.
+//
+//   out[t, n] = a_scale[t] * b_scale[e, n] * sum_k a[t, k] * b[e, n, k]  (+ bias[n])
+//   gated:      g, u the same with b and b2;  out = g / (1 + exp(-g)) * u
+//
+// for every row t of expert e's segment [offset_e, offset_e + count_e). The sums are exact:
+// tcgen05.mma kind::i8 accumulates in int32, and K <= 131071 keeps 128 * 128 * K below 2^31.
+// They are converted to fp32 once, scaled there, and rounded once more to the output type.
+//
+// Weight tiles are the MMA's M operand (128 output channels), tokens its N operand (TN), so a
+// decode step of a few tokens computes no padding beyond 16 columns and a TMEM lane holds one
+// output channel: the 32 lanes of a warp store 32 consecutive channels of one token, coalesced
+// for any width, alignment or row stride of the output, and no row outside a segment is
+// touched.
+//
+// Persistent CTAs walk tiles (expert, channel tile, token tile), token tiles fastest so that
+// tiles which share weights run together:
+//   warp 0     computes the tile ranges of the segments, then loads tiles by TMA (128-byte
+//              swizzle, zero fill past K and past the last row) into a ring of stages
+//   warp 1     TMEM allocation and the single-thread MMA issue (4 x K = 32 per stage)
+//   warps 2-5  epilogue: TMEM -> registers -> scales -> global
+// Accumulators are double-buffered in TMEM. Every wait is bounded in time (wait_phase).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "grouped_gemm_kernel.cuh"
+#include "sm100_ptx.cuh"
+
+namespace nvfp4 {
+
+constexpr int kInt8MaxExperts = 1024;
+constexpr int kInt8MaxK = 131071;
+constexpr int kInt8StageK = 128;  // bytes of K per stage: one 128-byte swizzle row
+constexpr int kInt8SegBytes = 3 * kInt8MaxExperts * 4;
+
+enum : int { kInt8OutBf16 = 0, kInt8OutFp16 = 1, kInt8OutFp32 = 2 };
+
+struct Int8GemmParams {
+  const float* a_scale;
+  const float* b_scale;
+  const float* b2_scale;
+  const float* bias;  // nullptr: none
+  void* out;
+  int64_t ldo;  // elements
+  const int32_t* seg_offsets;  // nullptr: one segment of all rows
+  const int32_t* seg_counts;
+  uint32_t* error_bits;
+  int32_t rows;
+  int32_t n;
+  int32_t ktiles;
+  int32_t num_experts;
+  int32_t out_dtype;
+};
+
+__device__ __forceinline__ void int8_store(void* out, int64_t i, float v, int dtype) {
+  if (dtype == kInt8OutBf16)
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else if (dtype == kInt8OutFp16)
+    static_cast<__half*>(out)[i] = __float2half_rn(v);
+  else
+    static_cast<float*>(out)[i] = v;
+}
+
+__device__ __forceinline__ float int8_silu_mul(float g, float u) {
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
+}
+
+// Segments of the launch in shared memory: first row, rows, and the end of each expert's tile
+// range. Warp-wide; a segment outside the slab is skipped and reported.
+__device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, int tile_rows,
+                                                    int n_tiles, int32_t* seg_row,
+                                                    int32_t* seg_cnt, int32_t* seg_end, int lane) {
+  int32_t carry = 0;
+  for (int base = 0; base < p.num_experts; base += 32) {
+    const int e = base + lane;
+    int32_t off = 0, cnt = 0;
+    if (e < p.num_experts) {
+      if (p.seg_offsets == nullptr) {
+        cnt = p.rows;
+      } else {
+        off = __ldg(p.seg_offsets + e);
+        cnt = __ldg(p.seg_counts + e);
+        if (cnt < 0 || off < 0 || static_cast<int64_t>(off) + cnt > p.rows) {
+          atomicOr(p.error_bits, kDevErrBadSegment);
+          off = cnt = 0;
+        }
+      }
+    }
+    int32_t v = (cnt + tile_rows - 1) / tile_rows * n_tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int32_t t = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += t;
+    }
+    if (e < p.num_experts) {
+      seg_row[e] = off;
+      seg_cnt[e] = cnt;
+      seg_end[e] = carry + v;
+    }
+    carry += __shfl_sync(0xffffffffu, v, 31);
+  }
+}
+
+struct Int8Tile {
+  int expert, row, rows, nt;  // rows: valid token rows of the tile
+};
+
+__device__ __forceinline__ Int8Tile int8_find_tile(int tile, int tile_rows, int n_tiles,
+                                                   int num_experts, const int32_t* seg_row,
+                                                   const int32_t* seg_cnt,
+                                                   const int32_t* seg_end) {
+  int lo = 0, hi = num_experts - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (seg_end[mid] > tile) hi = mid;
+    else lo = mid + 1;
+  }
+  const int cnt = seg_cnt[lo];
+  const int tiles_m = (cnt + tile_rows - 1) / tile_rows;
+  const int local = tile - (seg_end[lo] - tiles_m * n_tiles);
+  const int mt = local % tiles_m;
+  return {lo, seg_row[lo] + mt * tile_rows, min(tile_rows, cnt - mt * tile_rows), local / tiles_m};
+}
+
+template <int TN, bool GATED>
+struct Int8Config {
+  static constexpr int kSets = GATED ? 2 : 1;
+  static constexpr int kWBytes = 128 * kInt8StageK;
+  static constexpr int kXBytes = TN * kInt8StageK;
+  static constexpr int kStageBytes = kSets * kWBytes + kXBytes;
+  static constexpr int kFixedBytes = 1024 + kInt8SegBytes + 512;
+  static constexpr int kFit = (232448 - kFixedBytes) / kStageBytes;
+  static constexpr int kStages = kFit > 12 ? 12 : kFit;
+  static constexpr int kSmemBytes = kFixedBytes + kStages * kStageBytes;
+  static constexpr int kAccCols = TN * kSets;
+  static constexpr int kTmemColumns = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
+  static constexpr uint32_t kIdesc = ptx::make_idesc_i8(128, TN);
+  static_assert(kStages >= 3 && 8 * (2 * kStages + 5) + 16 <= 512, "shared memory layout");
+  static_assert((kTmemColumns & (kTmemColumns - 1)) == 0 && kTmemColumns <= 512, "TMEM columns");
+};
+
+template <int TN, bool GATED>
+__global__ void __launch_bounds__(kNumThreads, 1)
+    nvfp4_int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                           const __grid_constant__ CUtensorMap map_b,
+                           const __grid_constant__ CUtensorMap map_b2,
+                           const __grid_constant__ Int8GemmParams p) {
+  using Cfg = Int8Config<TN, GATED>;
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  int32_t* seg_row = reinterpret_cast<int32_t*>(smem + kStages * Cfg::kStageBytes);
+  int32_t* seg_cnt = seg_row + kInt8MaxExperts;
+  int32_t* seg_end = seg_cnt + kInt8MaxExperts;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(seg_end + kInt8MaxExperts);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* accf_bar = empty_bar + kStages;
+  uint64_t* acce_bar = accf_bar + 2;
+  uint64_t* drain_bar = acce_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile uint32_t* abort_flag = tmem_holder + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&full_bar[s], 1);
+      ptx::mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(&accf_bar[a], 1);
+      ptx::mbar_init(&acce_bar[a], kEpilogueWarps);
+    }
+    ptx::mbar_init(drain_bar, 1);
+    *abort_flag = 0u;
+    ptx::fence_mbarrier_init();
+    ptx::tma_prefetch_desc(&map_a);
+    ptx::tma_prefetch_desc(&map_b);
+    if (GATED) ptx::tma_prefetch_desc(&map_b2);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_holder, Cfg::kTmemColumns);
+    ptx::tmem_relinquish_alloc_permit();
+  }
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const int n_tiles = (p.n + 127) / 128;
+  if (warp == 0) int8_stage_segments(p, TN, n_tiles, seg_row, seg_cnt, seg_end, lane);
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  const int total = seg_end[p.num_experts - 1];
+  const int first = static_cast<int>(blockIdx.x);
+  const int step = static_cast<int>(gridDim.x);
+
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += step) {
+        const Int8Tile t =
+            int8_find_tile(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+        const int wrow = t.expert * p.n + t.nt * 128;
+        for (int kt = 0; kt < p.ktiles; ++kt) {
+          if (!wait_phase(&empty_bar[stage], phase ^ 1u, abort_flag, p.error_bits,
+                          kDevErrProducerTimeout)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sW = smem + stage * Cfg::kStageBytes;
+          ptx::mbar_arrive_expect_tx(&full_bar[stage], Cfg::kStageBytes);
+          ptx::tma_load_2d(sW, &map_b, &full_bar[stage], kt * kInt8StageK, wrow);
+          if (GATED)
+            ptx::tma_load_2d(sW + Cfg::kWBytes, &map_b2, &full_bar[stage], kt * kInt8StageK, wrow);
+          ptx::tma_load_2d(sW + Cfg::kSets * Cfg::kWBytes, &map_a, &full_bar[stage],
+                           kt * kInt8StageK, t.row);
+          ++issued;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // The most recent fill of each stage completes before the CTA may exit.
+      const uint32_t recent = issued < static_cast<uint32_t>(kStages) ? issued : kStages;
+      for (uint32_t i = 0; i < recent; ++i) {
+        const uint32_t n = issued - 1 - i;
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (!ptx::mbar_try_wait(&full_bar[n % kStages], (n / kStages) & 1u)) {
+          if (ptx::globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            atomicOr(p.error_bits, kDevErrDrainTimeout);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (ptx::elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t acc_parity = 0x3u;
+      uint32_t local = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += step, ++local) {
+        const int acc = static_cast<int>(local & 1u);
+        if (!wait_phase(&acce_bar[acc], (acc_parity >> acc) & 1u, abort_flag, p.error_bits,
+                        kDevErrAccTimeout))
+          break;
+        acc_parity ^= 1u << acc;
+        ptx::tcgen05_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + acc * Cfg::kAccCols;
+        for (int kt = 0; kt < p.ktiles; ++kt) {
+          if (!wait_phase(&full_bar[stage], phase, abort_flag, p.error_bits, kDevErrMmaTimeout)) {
+            ok = false;
+            break;
+          }
+          ptx::tcgen05_fence_after_sync();
+          const uint32_t sW = ptx::smem_u32(smem + stage * Cfg::kStageBytes);
+          const uint64_t w_desc = ptx::make_sw128_kmajor_desc(sW);
+          const uint64_t x_desc = ptx::make_sw128_kmajor_desc(sW + Cfg::kSets * Cfg::kWBytes);
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+            ptx::mma_i8(d_tmem, w_desc + 2 * kb, x_desc + 2 * kb, Cfg::kIdesc,
+                        (kt | kb) != 0 ? 1u : 0u);
+          if (GATED) {
+            const uint64_t w2_desc = ptx::make_sw128_kmajor_desc(sW + Cfg::kWBytes);
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+              ptx::mma_i8(d_tmem + TN, w2_desc + 2 * kb, x_desc + 2 * kb, Cfg::kIdesc,
+                          (kt | kb) != 0 ? 1u : 0u);
+          }
+          ptx::tcgen05_commit(&empty_bar[stage]);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        ptx::tcgen05_commit(&accf_bar[acc]);
+      }
+      ptx::tcgen05_commit(drain_bar);
+      const uint64_t t0 = ptx::globaltimer_ns();
+      while (!ptx::mbar_try_wait(drain_bar, 0)) {
+        if (ptx::globaltimer_ns() - t0 > kWaitTimeoutNs) {
+          atomicOr(p.error_bits, kDevErrDrainTimeout);
+          break;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    uint32_t full_parity = 0;
+    uint32_t local = 0;
+    for (int tile = first; tile < total; tile += step, ++local) {
+      const Int8Tile t =
+          int8_find_tile(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+      const int n = t.nt * 128 + 32 * quarter + lane;
+      const bool in = n < p.n;
+      const int64_t chan = static_cast<int64_t>(t.expert) * p.n + n;
+      const float bs = in ? __ldg(p.b_scale + chan) : 0.0f;
+      const float bs2 = GATED && in ? __ldg(p.b2_scale + chan) : 0.0f;
+      const float bias = !GATED && in && p.bias != nullptr ? __ldg(p.bias + n) : 0.0f;
+      const int acc = static_cast<int>(local & 1u);
+      if (!warp_wait_phase(&accf_bar[acc], (full_parity >> acc) & 1u, abort_flag, p.error_bits,
+                           kDevErrEpilogueTimeout, lane))
+        break;
+      full_parity ^= 1u << acc;
+      ptx::tcgen05_fence_after_sync();
+      const uint32_t t_acc =
+          tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) + acc * Cfg::kAccCols;
+      for (int c = 0; c < t.rows; c += 16) {
+        uint32_t v[16], u[16];
+        ptx::tmem_ld_32x32b_x16(t_acc + c, v);
+        if (GATED) ptx::tmem_ld_32x32b_x16(t_acc + TN + c, u);
+        ptx::tmem_ld_wait();
+        ptx::reg_fence(v);
+        if (GATED) ptx::reg_fence(u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (c + i >= t.rows) break;  // uniform over the warp
+          const int64_t row = static_cast<int64_t>(t.row) + c + i;
+          const float as = __ldg(p.a_scale + row);
+          float y = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(v[i])), as), bs);
+          if (GATED) {
+            const float w = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(u[i])), as), bs2);
+            y = int8_silu_mul(y, w);
+          } else {
+            y = __fadd_rn(y, bias);
+          }
+          if (in) int8_store(p.out, row * p.ldo + n, y, p.out_dtype);
+        }
+      }
+      ptx::tcgen05_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&acce_bar[acc]);
+    }
+  }
+  ptx::tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tcgen05_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, Cfg::kTmemColumns);
+  }
+}
+
+}  // namespace nvfp4

@@ -1,0 +1,258 @@
+// Host entry points of the int8 operators: the row quantiser and its dispatching form
+// (nvfp4_quantize_int8, nvfp4_moe_dispatch_int8) and the matrix product (nvfp4_int8_gemm).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/nvfp4_group_gemm.h"
+#include "host_common.cuh"
+#include "int8_gemm_kernel.cuh"
+#include "int8_quantize_kernel.cuh"
+
+namespace nvfp4 {
+
+// Why a product gave up on a wait or skipped a segment (kDevErr* bits), one word per device.
+// A product needs no workspace: its tensor maps travel as kernel parameters and nothing of one
+// call is left for the next, so calls on any streams and in any graphs may overlap.
+__device__ uint32_t g_int8_error_bits;
+
+namespace {
+
+struct Int8Device {
+  std::once_flag once;
+  cudaError_t status = cudaSuccess;
+  uint32_t* error_bits = nullptr;
+};
+Int8Device g_int8_dev[kMaxDevices];
+
+template <int TN, bool GATED>
+cudaError_t allow_smem() {
+  return cudaFuncSetAttribute(nvfp4_int8_gemm_kernel<TN, GATED>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Int8Config<TN, GATED>::kSmemBytes);
+}
+
+// Once per device. The look-up may load the module, which a stream capture under way on this
+// thread would otherwise forbid.
+void init_int8_device(Int8Device& d) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_int8_error_bits);
+  d.error_bits = static_cast<uint32_t*>(p);
+  if (e == cudaSuccess) e = allow_smem<16, false>();
+  if (e == cudaSuccess) e = allow_smem<32, false>();
+  if (e == cudaSuccess) e = allow_smem<64, false>();
+  if (e == cudaSuccess) e = allow_smem<128, false>();
+  if (e == cudaSuccess) e = allow_smem<16, true>();
+  if (e == cudaSuccess) e = allow_smem<32, true>();
+  if (e == cudaSuccess) e = allow_smem<64, true>();
+  if (e == cudaSuccess) e = allow_smem<128, true>();
+  d.status = e;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+}
+
+int int8_device(Int8Device** out, DeviceState** state) {
+  const int st = current_device_state(state);
+  if (st != NVFP4_OK) return st;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  Int8Device& d = g_int8_dev[dev];
+  std::call_once(d.once, init_int8_device, std::ref(d));
+  if (d.status != cudaSuccess) return cuda_fail(d.status, "int8 kernel set-up");
+  *out = &d;
+  return NVFP4_OK;
+}
+
+// int8 rows [rows, k], `ld` bytes apart, in boxes of 128 bytes x box_rows, 128-byte swizzle,
+// zero fill past the last column and row.
+bool int8_map(CUtensorMap* m, const void* addr, int64_t rows, int k, int64_t ld, int box_rows) {
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {kInt8StageK, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return encode_tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(addr), dims,
+                          strides, box, estr, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+template <int TN, bool GATED>
+int launch_int8(const nvfp4_int8_product* g, Int8GemmParams& p, int num_sms, cudaStream_t s) {
+  CUtensorMap ma, mb, mb2;
+  const int64_t wrows = static_cast<int64_t>(g->num_experts) * g->n;
+  if (!int8_map(&ma, g->a, g->rows, g->k, g->lda, TN) ||
+      !int8_map(&mb, g->b, wrows, g->k, g->ldb, 128) ||
+      !int8_map(&mb2, GATED ? g->b2 : g->b, wrows, g->k, g->ldb, 128))
+    return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
+  const int64_t n_tiles = (g->n + 127) / 128;
+  // The most tiles any segments can need: every row tile full, and one ragged tile each.
+  const int64_t tiles = ((g->rows + TN - 1) / TN + (g->num_experts - 1)) * n_tiles;
+  if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
+  const int64_t grid = std::min<int64_t>(tiles, num_sms);
+  const cudaError_t e =
+      launch_dependent(&nvfp4_int8_gemm_kernel<TN, GATED>, grid, kNumThreads,
+                       Int8Config<TN, GATED>::kSmemBytes, s, ma, mb, mb2, p);
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
+}
+
+template <bool GATED>
+int choose_int8(const nvfp4_int8_product* g, Int8GemmParams& p, int num_sms, cudaStream_t s) {
+  const int64_t expected = g->expected_rows > 0 ? std::min(g->expected_rows, g->rows) : g->rows;
+  const int64_t per_expert = (expected + g->num_experts - 1) / g->num_experts;
+  if (per_expert <= 16) return launch_int8<16, GATED>(g, p, num_sms, s);
+  if (per_expert <= 32) return launch_int8<32, GATED>(g, p, num_sms, s);
+  if (per_expert <= 64) return launch_int8<64, GATED>(g, p, num_sms, s);
+  return launch_int8<128, GATED>(g, p, num_sms, s);
+}
+
+int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
+                       const int32_t* row_mask, const int32_t* dest, int topk, int64_t out_rows,
+                       void* codes, int64_t codes_ld, float* scales, void* stream) {
+  if (dtype != NVFP4_DTYPE_BF16 && dtype != NVFP4_DTYPE_FP16)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "dtype=%d (expected NVFP4_DTYPE_BF16 or _FP16)", dtype);
+  if (rows < 0 || rows > 0x7fffffff || out_rows < 0 || out_rows > 0x7fffffff || cols <= 0)
+    return fail(NVFP4_ERR_BAD_SHAPE, "rows=%lld out_rows=%lld cols=%d", static_cast<long long>(rows),
+                static_cast<long long>(out_rows), cols);
+  if (rows == 0 || out_rows == 0) return NVFP4_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr)
+    return fail(NVFP4_ERR_NULL_POINTER, "x, codes or scales is NULL");
+  if (ld < cols || codes_ld < cols)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "ld=%lld codes_ld=%lld too small for cols=%d",
+                static_cast<long long>(ld), static_cast<long long>(codes_ld), cols);
+  if (!aligned16(codes) || codes_ld % 16 != 0)
+    return fail(NVFP4_ERR_MISALIGNED, "codes must be 16-byte aligned, codes_ld a multiple of 16");
+  DeviceState* ds = nullptr;
+  const int st = current_device_state(&ds);
+  if (st != NVFP4_OK) return st;
+  Int8QuantParams p = {};
+  p.x = static_cast<const uint16_t*>(x);
+  p.ld = ld;
+  p.rows = static_cast<int32_t>(rows);
+  p.cols = cols;
+  p.vec = aligned16(x) && ld % 8 == 0;
+  p.row_mask = row_mask;
+  p.dest = dest;
+  p.topk = topk;
+  p.out_rows = static_cast<int32_t>(out_rows);
+  p.codes = static_cast<int8_t*>(codes);
+  p.codes_ld = codes_ld;
+  p.scales = scales;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int per_thread = kInt8Chunk * kInt8ChunksPerThread;
+  const int need = (cols + per_thread - 1) / per_thread;  // threads that hold a row
+  auto go = [&](auto kernel, int group) {
+    const int64_t per_block = kInt8QuantThreads / group;
+    return launch_dependent(kernel, (rows + per_block - 1) / per_block, kInt8QuantThreads, 0, s, p);
+  };
+  cudaError_t e;
+  if (dtype == NVFP4_DTYPE_BF16)
+    e = need <= 32   ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 32>, 32)
+        : need <= 64 ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 64>, 64)
+        : need <= 128 ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 128>, 128)
+                      : go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 256>, 256);
+  else
+    e = need <= 32   ? go(&nvfp4_quantize_int8_kernel<__half, 32>, 32)
+        : need <= 64 ? go(&nvfp4_quantize_int8_kernel<__half, 64>, 64)
+        : need <= 128 ? go(&nvfp4_quantize_int8_kernel<__half, 128>, 128)
+                      : go(&nvfp4_quantize_int8_kernel<__half, 256>, 256);
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 quantiser launch");
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" {
+
+NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
+                                  const int32_t* row_mask, void* codes, int64_t codes_ld,
+                                  float* scales, void* stream) {
+  g_last_error.clear();
+  return quantize_int8_impl(x, rows, cols, ld, dtype, row_mask, nullptr, 1, rows, codes, codes_ld,
+                            scales, stream);
+}
+
+NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
+                                      const int32_t* dest, int topk, int64_t rows, void* codes,
+                                      int64_t codes_ld, float* scales, void* stream) {
+  g_last_error.clear();
+  if (topk <= 0 || static_cast<int64_t>(tokens) * topk > (int64_t{1} << 30))
+    return fail(NVFP4_ERR_BAD_SHAPE, "tokens=%d topk=%d", tokens, topk);
+  if (tokens > 0 && dest == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "dest is NULL");
+  return quantize_int8_impl(x, tokens, cols, ld, dtype, nullptr, dest, topk, rows, codes, codes_ld,
+                            scales, stream);
+}
+
+NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
+  g_last_error.clear();
+  if (g == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "product is NULL");
+  if (g->num_experts <= 0 || g->num_experts > kInt8MaxExperts)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "num_experts=%d must be in [1, %d]", g->num_experts,
+                kInt8MaxExperts);
+  if (g->out_dtype != NVFP4_DTYPE_BF16 && g->out_dtype != NVFP4_DTYPE_FP16 &&
+      g->out_dtype != NVFP4_DTYPE_FP32)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT,
+                "out_dtype=%d (expected NVFP4_DTYPE_BF16, _FP16 or _FP32)", g->out_dtype);
+  if (g->rows < 0 || g->rows > 0x7fffffff - 256 || g->n <= 0 || g->k <= 0 || g->k > kInt8MaxK ||
+      static_cast<int64_t>(g->num_experts) * g->n > 0x7fffffff - 256)
+    return fail(NVFP4_ERR_BAD_SHAPE, "rows=%lld n=%d k=%d (k in [1, %d])",
+                static_cast<long long>(g->rows), g->n, g->k, kInt8MaxK);
+  if ((g->seg_offsets == nullptr) != (g->seg_counts == nullptr))
+    return fail(NVFP4_ERR_NULL_POINTER, "seg_offsets and seg_counts must both be given or NULL");
+  if (g->seg_offsets == nullptr && g->num_experts != 1)
+    return fail(NVFP4_ERR_NULL_POINTER, "several experts need seg_offsets and seg_counts");
+  if ((g->b2 == nullptr) != (g->b2_scale == nullptr))
+    return fail(NVFP4_ERR_NULL_POINTER, "b2 and b2_scale must both be given or NULL");
+  const bool gated = g->b2 != nullptr;
+  if (g->bias != nullptr && (gated || g->num_experts != 1))
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "bias is for plain products of one weight matrix");
+  if (g->lda < g->k || g->ldb < g->k || g->ldo < g->n)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "lda/ldb < k or ldo < n");
+  if (g->rows == 0) return NVFP4_OK;
+  if (g->a == nullptr || g->a_scale == nullptr || g->b == nullptr || g->b_scale == nullptr ||
+      g->out == nullptr)
+    return fail(NVFP4_ERR_NULL_POINTER, "an operand, scale or output is NULL");
+  if (!aligned16(g->a) || !aligned16(g->b) || !aligned16(g->b2) || g->lda % 16 != 0 ||
+      g->ldb % 16 != 0)
+    return fail(NVFP4_ERR_MISALIGNED,
+                "operands must be 16-byte aligned, lda and ldb multiples of 16 bytes");
+  Int8Device* d = nullptr;
+  DeviceState* ds = nullptr;
+  const int st = int8_device(&d, &ds);
+  if (st != NVFP4_OK) return st;
+  Int8GemmParams p = {};
+  p.a_scale = g->a_scale;
+  p.b_scale = g->b_scale;
+  p.b2_scale = g->b2_scale;
+  p.bias = g->bias;
+  p.out = g->out;
+  p.ldo = g->ldo;
+  p.seg_offsets = g->seg_offsets;
+  p.seg_counts = g->seg_counts;
+  p.error_bits = d->error_bits;
+  p.rows = static_cast<int32_t>(g->rows);
+  p.n = g->n;
+  p.ktiles = (g->k + kInt8StageK - 1) / kInt8StageK;
+  p.num_experts = g->num_experts;
+  p.out_dtype = g->out_dtype == NVFP4_DTYPE_BF16   ? kInt8OutBf16
+                : g->out_dtype == NVFP4_DTYPE_FP16 ? kInt8OutFp16
+                                                   : kInt8OutFp32;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return gated ? choose_int8<true>(g, p, ds->num_sms, s) : choose_int8<false>(g, p, ds->num_sms, s);
+}
+
+NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits) {
+  g_last_error.clear();
+  if (device_error_bits) *device_error_bits = 0;
+  Int8Device* d = nullptr;
+  DeviceState* ds = nullptr;
+  const int st = int8_device(&d, &ds);
+  if (st != NVFP4_OK) return st;
+  return nvfp4_workspace_check(d->error_bits, stream, device_error_bits);
+}
+
+}  // extern "C"

@@ -347,6 +347,21 @@ void init_encoder(Encoder& e) {
   if (err == cudaSuccess && q == cudaDriverEntryPointSuccess) e.fn = reinterpret_cast<EncodeFn>(fn);
 }
 
+}  // namespace
+
+bool encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, unsigned rank, void* addr,
+                      const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                      const cuuint32_t* elem_strides, CUtensorMapSwizzle swizzle,
+                      CUtensorMapL2promotion promotion) {
+  std::call_once(g_encoder.once, init_encoder, std::ref(g_encoder));
+  return g_encoder.fn != nullptr &&
+         g_encoder.fn(map, type, rank, addr, dims, strides, box, elem_strides,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
 // Encoded maps are cached by (kind, address, rows, row elements): weights keep
 // their maps across calls, so steady-state calls encode only what changed.
 struct MapKey {

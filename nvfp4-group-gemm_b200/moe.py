@@ -31,7 +31,11 @@ import torch
 from . import _native
 from .interface import grouped_gemm_table
 from .layout import blocked_sf_bytes
+from .int8 import _check_activations, _check_code_outputs, _codes_stride, _launch_on, _row_stride
+from .int8 import check_int8_errors, empty_codes, int8_gemm_segments, quantize_int8
 from .quantize import _DTYPES, global_scale_for, quantize
+from .token_sort import (combine_tokens, combine_tokens_backward, dispatch_tokens,  # noqa: F401
+                         dispatch_tokens_backward)
 
 
 @dataclass
@@ -133,6 +137,36 @@ def combine(y: torch.Tensor, routing: Routing, topk_weights: torch.Tensor,
                                             w.data_ptr(), routing.tokens, routing.topk, cols,
                                             out.data_ptr(), out.stride(0), s.cuda_stream), lib)
     return out
+
+
+def dispatch_int8(x: torch.Tensor, routing: Routing, codes: torch.Tensor | None = None,
+                  scales: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> tuple:
+    """:func:`quantize_int8` of each token straight into its experts' rows: ``(codes, scales)``
+    of ``routing.rows`` rows in dispatched order, each token read and quantised once. Padding
+    rows are not written (the products do not read them either)."""
+    _check_activations(x)
+    if int(x.shape[0]) != routing.tokens:
+        raise ValueError(f"x must have {routing.tokens} rows, got {int(x.shape[0])}")
+    rows, cols = routing.rows, int(x.shape[1])
+    dest = routing.dest
+    if dest.dtype != torch.int32 or not dest.is_contiguous() or \
+            dest.numel() < routing.tokens * routing.topk:
+        raise ValueError(f"routing.dest must be contiguous int32 with "
+                         f"{routing.tokens * routing.topk} entries")
+    _check_code_outputs(codes, scales, rows, cols)
+    s, where = _launch_on((x, dest, codes, scales), stream)
+    with where:
+        if codes is None:
+            codes = empty_codes(rows, cols, x.device)
+        if scales is None:
+            scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        lib = _native.load_library()
+        _native.check(lib.nvfp4_moe_dispatch_int8(
+            x.data_ptr(), routing.tokens, cols, _row_stride(x), _DTYPES[x.dtype], dest.data_ptr(),
+            routing.topk, rows, codes.data_ptr(), _codes_stride(codes, "codes"),
+            scales.data_ptr(), s.cuda_stream), lib)
+    return codes, scales
 
 
 def expert_views(routing: Routing, packed: torch.Tensor, sf: torch.Tensor, out: torch.Tensor,
@@ -426,6 +460,151 @@ class MoEBlock:
         """Record one run over these input tensors into a CUDA graph (after ``warmup`` eager
         runs, which upload the GEMMs' descriptors so the graph holds only their launches).
         ``graph.replay()`` then recomputes ``self.out`` from the tensors' current contents."""
+        side = torch.cuda.Stream(self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(side):
+            for _ in range(max(warmup, 1)):
+                self.run(x, topk_ids, topk_weights, side)
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            self.run(x, topk_ids, topk_weights, side)
+        return graph
+
+
+@dataclass
+class Int8ExpertWeights:
+    """int8 weights of the experts, a scale per output channel: gate/up codes [E, I, H] with
+    scales [E, I], down codes [E, H, I] with scales [E, H] (rows a multiple of 16 bytes apart)."""
+
+    w_gate: torch.Tensor
+    s_gate: torch.Tensor
+    w_up: torch.Tensor
+    s_up: torch.Tensor
+    w_down: torch.Tensor
+    s_down: torch.Tensor
+
+    @property
+    def num_experts(self) -> int:
+        return int(self.w_gate.shape[0])
+
+
+def quantize_expert_weights_int8(gate, up, down) -> Int8ExpertWeights:
+    """Quantise bf16/fp16 expert weights (gate/up [I, H], down [H, I] per expert: lists or stacked
+    tensors) to int8 codes with a scale per output channel."""
+    out = []
+    for name, ws in (("gate", gate), ("up", up), ("down", down)):
+        rows, cols = int(ws[0].shape[0]), int(ws[0].shape[1])
+        E = len(ws)
+        codes = empty_codes(E * rows, cols, ws[0].device)
+        scales = torch.empty((E, rows), dtype=torch.float32, device=ws[0].device)
+        for e, w in enumerate(ws):
+            if tuple(w.shape) != (rows, cols):
+                raise ValueError(f"{name}[{e}] is {list(w.shape)}, {name}[0] is {[rows, cols]}")
+            quantize_int8(w, codes[e * rows:(e + 1) * rows], scales[e])
+        out += [codes.unflatten(0, (E, rows)), scales]
+    return Int8ExpertWeights(*out)
+
+
+class Int8MoEBlock:
+    """The MoE feed-forward block in int8 with a scale per token and per channel, over buffers
+    sized once for ``tokens`` x ``topk``, with no device -> host read in :meth:`run`:
+
+        x --route--> rows --quantise+dispatch--> codes --gated product--> h
+          --quantise (a scale per row)--> codes --product (down)--> y --weighted combine--> out
+
+    Activations are quantised from the data of every run (no calibrated scales, unlike
+    :class:`MoEBlock`). ``x``, h, y and ``out`` have the type ``dtype`` (bf16 or fp16); hidden and
+    intermediate sizes may be anything. :meth:`run` returns ``self.out`` [tokens, H], overwritten
+    by the next run; :meth:`capture` records a run in a CUDA graph.
+    """
+
+    def __init__(self, weights: Int8ExpertWeights, tokens: int, topk: int,
+                 dtype: torch.dtype = torch.bfloat16):
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
+        if tokens <= 0 or topk <= 0:
+            raise ValueError("tokens and topk must be positive")
+        E, idim, hdim = (int(v) for v in weights.w_gate.shape)
+        if tuple(weights.w_up.shape) != (E, idim, hdim) or \
+                tuple(weights.w_down.shape) != (E, hdim, idim):
+            raise ValueError("w_gate and w_up must be [E, I, H], w_down [E, H, I]")
+        dev = weights.w_gate.device
+        self.tokens, self.topk, self.num_experts = tokens, topk, E
+        self.hidden, self.intermediate, self.dtype, self.device = hdim, idim, dtype, dev
+        pairs = tokens * topk
+        cap = self.capacity = pairs + 127 * E
+        i32 = dict(dtype=torch.int32, device=dev)
+        f32 = dict(dtype=torch.float32, device=dev)
+        self._meta = torch.zeros(2 * E + 1, **i32)
+        self.counts, self.offsets = self._meta[:E], self._meta[E:]
+        self.dest = torch.empty(pairs, **i32)
+        self.src_rows = torch.empty(cap, **i32)
+        lib = self._lib = _native.load_library()
+        self._route_ws_bytes = int(lib.nvfp4_moe_route_workspace_size(pairs, E))
+        self._route_ws = torch.empty(max(self._route_ws_bytes, 16), dtype=torch.uint8, device=dev)
+        self._a, self._a_scale = empty_codes(cap, hdim, dev), torch.empty(cap, **f32)
+        self._h = torch.empty((cap, idim), dtype=dtype, device=dev)
+        self._a2, self._a2_scale = empty_codes(cap, idim, dev), torch.empty(cap, **f32)
+        self._y = torch.empty((cap, hdim), dtype=dtype, device=dev)
+        self._w = torch.empty((tokens, topk), **f32)
+        self.out = torch.empty((tokens, hdim), dtype=dtype, device=dev)
+        self._weights = weights
+
+    def _check_inputs(self, x, topk_ids, topk_weights):
+        if x.dtype != self.dtype or tuple(x.shape) != (self.tokens, self.hidden) or \
+                x.stride(1) != 1 or x.device != self.device:
+            raise ValueError(f"x must be {self.dtype} [{self.tokens}, {self.hidden}] on {self.device}")
+        if topk_ids.dtype != torch.int32 or tuple(topk_ids.shape) != (self.tokens, self.topk) or \
+                not topk_ids.is_contiguous() or topk_ids.device != self.device:
+            raise ValueError(f"topk_ids must be contiguous int32 [{self.tokens}, {self.topk}]")
+        if tuple(topk_weights.shape) != (self.tokens, self.topk) or \
+                topk_weights.device != self.device:
+            raise ValueError(f"topk_weights must be [{self.tokens}, {self.topk}]")
+
+    def run(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+            stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """One block on ``stream``."""
+        self._check_inputs(x, topk_ids, topk_weights)
+        st = stream or torch.cuda.current_stream(self.device)
+        s = st.cuda_stream
+        lib, chk = self._lib, _native.check
+        T, K, E, cap, W = self.tokens, self.topk, self.num_experts, self.capacity, self._weights
+        with torch.cuda.device(self.device):
+            chk(lib.nvfp4_moe_route(topk_ids.data_ptr(), T, K, E, self.counts.data_ptr(),
+                                    self.offsets.data_ptr(), self.dest.data_ptr(),
+                                    self.src_rows.data_ptr(), cap, self._route_ws.data_ptr(),
+                                    self._route_ws_bytes, s), lib)
+            chk(lib.nvfp4_moe_dispatch_int8(x.data_ptr(), T, self.hidden, _row_stride(x),
+                                            _DTYPES[x.dtype], self.dest.data_ptr(), K, cap,
+                                            self._a.data_ptr(), self._a.stride(0),
+                                            self._a_scale.data_ptr(), s), lib)
+            int8_gemm_segments(self._a, self._a_scale, W.w_gate, W.s_gate, self.offsets, self.counts,
+                               b2=W.w_up, b2_scale=W.s_up, out=self._h, expected_rows=T * K,
+                               stream=st)
+            quantize_int8(self._h, self._a2, self._a2_scale, row_mask=self.src_rows, stream=st)
+            int8_gemm_segments(self._a2, self._a2_scale, W.w_down, W.s_down, self.offsets,
+                               self.counts, out=self._y, expected_rows=T * K, stream=st)
+            w = topk_weights
+            if w.dtype != torch.float32 or not w.is_contiguous():
+                with torch.cuda.stream(st):
+                    self._w.copy_(w)
+                w = self._w
+            chk(lib.nvfp4_moe_combine_tokens(self._y.data_ptr(), self._y.stride(0),
+                                             _DTYPES[self.dtype], self.dest.data_ptr(),
+                                             w.data_ptr(), T, K, self.hidden, cap,
+                                             self.out.data_ptr(), self.out.stride(0), s), lib)
+        return self.out
+
+    def check_device_errors(self) -> int:
+        """Synchronise and return the device error bits of the int8 products (raises Nvfp4Error
+        when a segment was out of range or a wait timed out)."""
+        return check_int8_errors(self.device)
+
+    def capture(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+                warmup: int = 1) -> torch.cuda.CUDAGraph:
+        """Record one run over these input tensors into a CUDA graph (after ``warmup`` eager
+        runs); ``graph.replay()`` recomputes ``self.out`` from their current contents."""
         side = torch.cuda.Stream(self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):

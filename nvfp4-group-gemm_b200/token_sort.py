@@ -1,0 +1,196 @@
+"""Tokens sorted by expert and back, with weights applied, and the gradients of both.
+
+    r = moe.route(topk_ids, num_experts)
+    rows = dispatch_tokens(x, r)                 # [r.rows, H], every expert's rows together
+    ...                                          # the experts
+    out = combine_tokens(rows, r, topk_weights)  # [tokens, H]
+
+bf16, fp16 and fp32, any width and row stride, differentiable (first order) in ``x``, the rows
+and the weights. Sums are fp32 in slot order, rounded once: results do not depend on timing.
+The ``*_backward`` functions are the gradients by themselves, for training loops that do not go
+through autograd. The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from .int8 import _OUT_DTYPES, _launch_on, _row_stride, _unit_inner
+
+
+def _check_routing(routing) -> tuple:
+    """``(tokens, topk, rows, dest, src_rows)`` of a Routing, checked against one another."""
+    tokens, topk, rows = int(routing.tokens), int(routing.topk), int(routing.rows)
+    dest, src = routing.dest, routing.src_rows
+    if dest.dtype != torch.int32 or dest.numel() < tokens * topk or not dest.is_contiguous():
+        raise ValueError(f"routing.dest must be contiguous int32 with {tokens * topk} entries")
+    if src.dtype != torch.int32 or src.numel() < rows or not src.is_contiguous():
+        raise ValueError(f"routing.src_rows must be contiguous int32 with >= {rows} entries")
+    return tokens, topk, rows, dest, src
+
+
+def _check_rows(t: torch.Tensor, rows: int, name: str, cols: int | None = None) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _OUT_DTYPES:
+        raise ValueError(f"{name} must be a CUDA bf16, fp16 or fp32 tensor")
+    if t.dim() != 2 or int(t.shape[0]) != rows or t.shape[1] < 1 or \
+            (cols is not None and int(t.shape[1]) != cols):
+        want = f"[{rows}, {'cols' if cols is None else cols}]"
+        raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy where its rows overlap (expanded tensors) or are not contiguous."""
+    if not _unit_inner(t) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _dispatch(x, routing, stream):
+    tokens, topk, rows, dest, src = _check_routing(routing)
+    _check_rows(x, tokens, "x")
+    s, where = _launch_on((x, dest, src), stream)
+    with where:
+        x = _rows_of(x)
+        cols = int(x.shape[1])
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        lib = _native.load_library()
+        _native.check(lib.nvfp4_moe_dispatch_tokens(
+            x.data_ptr(), _row_stride(x), _OUT_DTYPES[x.dtype], dest.data_ptr(), src.data_ptr(),
+            tokens, topk, cols, rows, y.data_ptr(), cols, s.cuda_stream), lib)
+    return y
+
+
+def _check_weights(weights, tokens, topk):
+    if tuple(weights.shape) != (tokens, topk) or not weights.is_floating_point():
+        raise ValueError(f"weights must be a floating-point tensor [{tokens}, {topk}]")
+
+
+def _combine(y, routing, weights, stream):
+    tokens, topk, rows, dest, _ = _check_routing(routing)
+    _check_rows(y, rows, "y")
+    if weights is not None:
+        _check_weights(weights, tokens, topk)
+    s, where = _launch_on((y, dest, weights), stream)
+    with where:
+        y = _rows_of(y)
+        w = weights.to(torch.float32).contiguous() if weights is not None else None
+        cols = int(y.shape[1])
+        out = torch.empty((tokens, cols), dtype=y.dtype, device=y.device)
+        lib = _native.load_library()
+        _native.check(lib.nvfp4_moe_combine_tokens(
+            y.data_ptr(), _row_stride(y), _OUT_DTYPES[y.dtype], dest.data_ptr(), _ptr(w), tokens,
+            topk, cols, rows, out.data_ptr(), cols, s.cuda_stream), lib)
+    return out
+
+
+def dispatch_tokens_backward(grad_y: torch.Tensor, routing,
+                             stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Gradient of :func:`dispatch_tokens`: ``grad_x[t] = sum_j grad_y[dest[t, j]]``."""
+    return _combine(grad_y, routing, None, stream)
+
+
+def combine_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor | None, routing,
+                            weights: torch.Tensor | None = None, want_y: bool = True,
+                            want_weights: bool = True,
+                            stream: torch.cuda.Stream | None = None) -> tuple:
+    """Gradients of :func:`combine_tokens`: ``(grad_y, grad_weights)``, None for one not wanted.
+
+    ``grad_y[dest[t, j]] = weights[t, j] * grad_out[t]`` (zeros on padding rows) in the type of
+    ``grad_out``; ``grad_weights[t, j] = <grad_out[t], y[dest[t, j]]>`` in fp32 (0 for dropped
+    pairs; ``y`` is needed for it).
+    """
+    tokens, topk, rows, dest, src = _check_routing(routing)
+    _check_rows(grad_out, tokens, "grad_out")
+    cols = int(grad_out.shape[1])
+    if want_weights:
+        if y is None:
+            raise ValueError("the gradient of the weights needs y")
+        _check_rows(y, rows, "y", cols)
+        if y.dtype != grad_out.dtype:
+            raise ValueError(f"y is {y.dtype}, grad_out is {grad_out.dtype}")
+    if weights is not None:
+        _check_weights(weights, tokens, topk)
+    used_y = y if want_weights else None
+    s, where = _launch_on((grad_out, dest, src, weights, used_y), stream)
+    with where:
+        g = _rows_of(grad_out)
+        used_y = _rows_of(used_y) if want_weights else None
+        w = weights.to(torch.float32).contiguous() if weights is not None else None
+        dev = g.device
+        gy = torch.empty((rows, cols), dtype=g.dtype, device=dev) if want_y else None
+        gw = torch.empty((tokens, topk), dtype=torch.float32, device=dev) if want_weights else None
+        lib = _native.load_library()
+        _native.check(lib.nvfp4_moe_combine_tokens_backward(
+            g.data_ptr(), _row_stride(g), _ptr(used_y), _row_stride(used_y) if want_weights else 0,
+            _OUT_DTYPES[g.dtype], dest.data_ptr(), src.data_ptr(), _ptr(w), tokens, topk, cols, rows,
+            _ptr(gy), cols, _ptr(gw), s.cuda_stream), lib)
+    return gy, gw
+
+
+class _Kept:
+    """The parts of a Routing a gradient needs (its tensors come back from the saved ones)."""
+
+    def __init__(self, routing, dest, src_rows):
+        self.tokens, self.topk, self.rows = int(routing.tokens), int(routing.topk), int(routing.rows)
+        self.dest, self.src_rows = dest, src_rows
+
+
+class _DispatchTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, routing):
+        ctx.routing = _Kept(routing, None, None)
+        ctx.save_for_backward(routing.dest, routing.src_rows)
+        return _dispatch(x, routing, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        ctx.routing.dest, ctx.routing.src_rows = ctx.saved_tensors
+        return dispatch_tokens_backward(grad_y, ctx.routing), None
+
+
+class _CombineTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, routing):
+        want_w = weights is not None and ctx.needs_input_grad[1]
+        ctx.routing = _Kept(routing, None, None)
+        ctx.save_for_backward(routing.dest, routing.src_rows, weights, y if want_w else None)
+        return _combine(y, routing, weights, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        dest, src, weights, y = ctx.saved_tensors
+        ctx.routing.dest, ctx.routing.src_rows = dest, src
+        gy, gw = combine_tokens_backward(grad_out, y, ctx.routing, weights,
+                                         want_y=ctx.needs_input_grad[0], want_weights=y is not None)
+        return gy, gw.to(weights.dtype) if gw is not None else None, None
+
+
+def dispatch_tokens(x: torch.Tensor, routing,
+                    stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Tokens in expert order: ``[routing.rows, H]`` with ``y[routing.dest[t, j]] = x[t]`` and
+    zeros on every expert's padding rows; differentiable in ``x`` (bf16, fp16 or fp32)."""
+    if stream is None:
+        return _DispatchTokens.apply(x, routing)
+    _launch_on((x, routing.dest, routing.src_rows), stream)
+    with torch.cuda.stream(stream):  # the backward pass runs on the stream of the forward pass
+        return _DispatchTokens.apply(x, routing)
+
+
+def combine_tokens(y: torch.Tensor, routing, weights: torch.Tensor | None = None,
+                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * y[routing.dest[t, j]]`` (``weights`` None: ones), ``y``
+    bf16, fp16 or fp32 ``[routing.rows, H]``, the result in its type; dropped pairs add nothing.
+    Products and sums are fp32. Differentiable in ``y`` and ``weights``. (:func:`moe.combine` is
+    the inference form from fp16 rows to bf16.)"""
+    if stream is None:
+        return _CombineTokens.apply(y, weights, routing)
+    _launch_on((y, routing.dest, routing.src_rows, weights), stream)
+    with torch.cuda.stream(stream):
+        return _CombineTokens.apply(y, weights, routing)

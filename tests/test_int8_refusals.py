@@ -1,0 +1,120 @@
+"""What the int8 operators and the token sort refuse, before anything is launched (CPU only)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+
+def _product(N, **kw):
+    p = N.Int8Product()
+    base = dict(a=0x10000, b=0x20000, a_scale=0x30000, b_scale=0x40000, out=0x50000, rows=16, n=64,
+                k=100, lda=112, ldb=112, ldo=64, num_experts=1, out_dtype=0)
+    base.update(kw)
+    for k, v in base.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(k=0), 2), (dict(k=131072, lda=131072, ldb=131072), 2), (dict(n=0), 2), (dict(rows=-1), 2),
+    (dict(rows=2 ** 31), 2), (dict(n=2 ** 30, num_experts=4, ldo=2 ** 30, seg_offsets=0x100, seg_counts=0x200), 2),
+    (dict(num_experts=0), 1), (dict(num_experts=1025), 1), (dict(out_dtype=3), 1), (dict(out_dtype=-1), 1),
+    (dict(num_experts=2), 4), (dict(seg_offsets=0x100), 4), (dict(b2=0x60000), 4),
+    (dict(a=0), 4), (dict(b_scale=0), 4), (dict(out=0), 4),
+    (dict(bias=0x100, b2=0x60000, b2_scale=0x70000), 1),
+    (dict(lda=96), 1), (dict(ldb=96), 1), (dict(ldo=63), 1),
+    (dict(lda=120), 3), (dict(ldb=104), 3), (dict(a=0x10008), 3), (dict(b=0x20001), 3),
+])
+def test_product_statuses(pkg, kw, status):
+    lib = pkg.load_library()
+    assert lib.nvfp4_int8_gemm(ctypes.byref(_product(pkg._native, **kw)), None) == status
+    assert lib.nvfp4_last_error_detail()
+
+
+def test_product_of_no_rows_and_null(pkg):
+    lib = pkg.load_library()
+    assert lib.nvfp4_int8_gemm(ctypes.byref(_product(pkg._native, rows=0)), None) == 0
+    assert lib.nvfp4_int8_gemm(None, None) == 4
+
+
+def test_product_struct_layout(pkg):
+    P = pkg._native.Int8Product
+    assert ctypes.sizeof(P) == 10 * 8 + 5 * 8 + 4 * 4
+    assert P.rows.offset == 80 and P.n.offset == 120
+
+
+def test_quantiser_statuses(pkg):
+    lib = pkg.load_library()
+
+    def call(x=0x1000, rows=4, cols=33, ld=33, dtype=0, mask=None, codes=0x2000, codes_ld=48, scales=0x3000):
+        return lib.nvfp4_quantize_int8(x, rows, cols, ld, dtype, mask, codes, codes_ld, scales, None)
+
+    assert call(dtype=2) == 1 and call(dtype=-1) == 1
+    assert call(cols=0) == 2 and call(rows=-1) == 2 and call(rows=2 ** 31) == 2
+    assert call(x=None) == 4 and call(codes=None) == 4 and call(scales=None) == 4
+    assert call(ld=32) == 1 and call(codes_ld=32) == 1
+    assert call(codes=0x2008) == 3 and call(codes_ld=40) == 3
+    assert call(rows=0) == 0
+
+    def dispatch(tokens=4, topk=2, dest=0x4000, rows=128, cols=33):
+        return lib.nvfp4_moe_dispatch_int8(0x1000, tokens, cols, 33, 0, dest, topk, rows, 0x2000, 48, 0x3000, None)
+
+    assert dispatch(topk=0) == 2 and dispatch(tokens=2 ** 30) == 2 and dispatch(rows=-1) == 2
+    assert dispatch(dest=None) == 4 and dispatch(tokens=0) == 0 and dispatch(rows=0) == 0
+
+
+def test_token_sort_statuses(pkg):
+    lib = pkg.load_library()
+
+    def disp(x=0x1000, ldx=8, dtype=0, dest=0x2000, src=0x3000, tokens=4, topk=2, cols=8, rows=128, y=0x4000, ldy=8):
+        return lib.nvfp4_moe_dispatch_tokens(x, ldx, dtype, dest, src, tokens, topk, cols, rows, y, ldy, None)
+
+    assert disp(dtype=3) == 1 and disp(ldx=7) == 1 and disp(ldy=7) == 1
+    assert disp(tokens=-1) == 2 and disp(topk=0) == 2 and disp(cols=0) == 2 and disp(rows=2 ** 31) == 2
+    assert disp(x=None) == 4 and disp(dest=None) == 4 and disp(src=None) == 4 and disp(y=None) == 4
+    assert disp(rows=0) == 0
+
+    def comb(y=0x1000, ldy=8, dtype=0, dest=0x2000, w=None, tokens=4, topk=2, cols=8, rows=128, out=0x4000, ldo=8):
+        return lib.nvfp4_moe_combine_tokens(y, ldy, dtype, dest, w, tokens, topk, cols, rows, out, ldo, None)
+
+    assert comb(dtype=-1) == 1 and comb(ldy=7) == 1 and comb(ldo=7) == 1 and comb(rows=-1) == 2
+    assert comb(y=None) == 4 and comb(out=None) == 4 and comb(tokens=0) == 0
+
+    def back(g=0x1000, ldg=8, y=0x2000, ldy=8, dtype=0, dest=0x3000, src=0x4000, w=None, tokens=4, topk=2, cols=8,
+             rows=128, gy=0x5000, ldo=8, gw=0x6000):
+        return lib.nvfp4_moe_combine_tokens_backward(g, ldg, y, ldy, dtype, dest, src, w, tokens, topk, cols, rows,
+                                                     gy, ldo, gw, None)
+
+    assert back(dtype=7) == 1 and back(ldg=7) == 1 and back(ldy=7) == 1 and back(ldo=7) == 1
+    assert back(g=None) == 4 and back(y=None) == 4 and back(src=None) == 4
+    assert back(gy=None, gw=None) == 0 and back(cols=-1) == 2
+
+
+def test_python_checks_refuse_cpu_tensors_and_bad_types(pkg):
+    x = torch.zeros((4, 32), dtype=torch.bfloat16)
+    q = torch.zeros((4, 32), dtype=torch.int8)
+    s = torch.zeros(4)
+    for call in (lambda: pkg.quantize_int8(x), lambda: pkg.int8_gemm(q, s, q, s),
+                 lambda: pkg.int8_gemm_segments(q, s, q[None], s[None], s.int(), s.int())):
+        with pytest.raises(ValueError):
+            call()
+    r = pkg.moe.Routing(4, 1, 1, [4], [0, 128], torch.zeros(4, dtype=torch.int32),
+                        torch.zeros(128, dtype=torch.int32))
+    for call in (lambda: pkg.moe.dispatch_tokens(x, r), lambda: pkg.moe.combine_tokens(x, r),
+                 lambda: pkg.moe.dispatch_int8(x, r), lambda: pkg.moe.combine_tokens_backward(x, x, r)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_block_refuses_bad_sizes(pkg):
+    w = pkg.moe.Int8ExpertWeights(*(torch.zeros(s, dtype=t) for s, t in (
+        ((2, 8, 16), torch.int8), ((2, 8), torch.float32), ((2, 8, 16), torch.int8), ((2, 8), torch.float32),
+        ((2, 16, 9), torch.int8), ((2, 16), torch.float32))))
+    with pytest.raises(ValueError, match="w_down"):
+        pkg.moe.Int8MoEBlock(w, 4, 2)
+    with pytest.raises(ValueError, match="positive"):
+        pkg.moe.Int8MoEBlock(w, 0, 2)
+    with pytest.raises(ValueError, match="dtype"):
+        pkg.moe.Int8MoEBlock(w, 4, 2, dtype=torch.float32)
