@@ -18,7 +18,8 @@ SOURCES = ["nvfp4_group_gemm.cu", "moe_host.cu", "ep_host.cu", "int8_host.cu",
            "token_sort_host.cu"]
 HEADERS = ["grouped_gemm_kernel.cuh", "grouped_gemm_pair_kernel.cuh", "grouped_gemm_swap_kernel.cuh",
            "quantize_kernel.cuh", "moe_kernels.cuh", "nvfp4_quant_math.cuh", "ep_kernels.cuh",
-           "row_ops.cuh", "host_common.cuh", "int8_gemm_kernel.cuh", "int8_quantize_kernel.cuh",
+           "row_ops.cuh", "host_common.cuh", "int8_gemm_kernel.cuh",
+           "int8_gemm_pair_kernel.cuh", "int8_gemv_kernel.cuh", "int8_quantize_kernel.cuh",
            "token_sort_kernels.cuh",
            "nvfp4_types.cuh", "sm100_ptx.cuh"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(HERE), "include", "nvfp4_group_gemm.h")

@@ -31,9 +31,10 @@ bool encode_tiled_map(CUtensorMap* map, CUtensorMapDataType type, unsigned rank,
 
 // Launch with programmatic stream serialization: the kernel may be scheduled while its
 // predecessor in the stream drains, and must run griddepcontrol.wait before it touches memory.
+// `grid` is a multiple of `cluster`, the CTAs per cluster.
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, int smem,
-                             cudaStream_t stream, const Args&... args) {
+cudaError_t launch_clusters(void (*kernel)(Params...), int64_t grid, int cluster, int threads,
+                            int smem, cudaStream_t stream, const Args&... args) {
   if (grid <= 0) return cudaSuccess;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
@@ -41,12 +42,21 @@ cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int thread
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, int smem,
+                             cudaStream_t stream, const Args&... args) {
+  return launch_clusters(kernel, grid, 1, threads, smem, stream, args...);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -7,24 +7,27 @@
 // tcgen05.mma kind::i8 accumulates in int32, and K <= 131071 keeps 128 * 128 * K below 2^31.
 // They are converted to fp32 once, scaled there, and rounded once more to the output type.
 //
-// Weight tiles are the MMA's M operand (128 output channels), tokens its N operand (TN), so a
-// decode step of a few tokens computes no padding beyond 16 columns and a TMEM lane holds one
-// output channel: the 32 lanes of a warp store 32 consecutive channels of one token, coalesced
-// for any width, alignment or row stride of the output, and no row outside a segment is
-// touched.
+// Weight rows are the MMA's M operand, tokens its N operand, so a decode step of a few tokens
+// computes no padding beyond 16 columns, and a TMEM lane holds one output channel: the 32
+// lanes of a warp store 32 consecutive channels of one token, coalesced for any width,
+// alignment or row stride of the output, and no row outside a segment is touched.
 //
 // Persistent CTAs walk tiles (expert, channel tile, token tile), token tiles fastest so that
 // tiles which share weights run together:
 //   warp 0     computes the tile ranges of the segments, then loads tiles by TMA (128-byte
 //              swizzle, zero fill past K and past the last row) into a ring of stages
 //   warp 1     TMEM allocation and the single-thread MMA issue (4 x K = 32 per stage)
-//   warps 2-5  epilogue: TMEM -> registers -> scales -> global
+//   warps 2..  epilogue: TMEM -> registers -> scales -> global (4 warps, or 8 for tiles of 64
+//              or more tokens, the second four taking the upper half of the tokens: with 4
+//              the stores of a tile took longer than its MMAs at K = 1536)
 // Accumulators are double-buffered in TMEM. Every wait is bounded in time (wait_phase).
 #pragma once
 
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "grouped_gemm_kernel.cuh"
 #include "sm100_ptx.cuh"
@@ -53,15 +56,62 @@ struct Int8GemmParams {
   int32_t ktiles;
   int32_t num_experts;
   int32_t out_dtype;
+  int32_t out_vec;  // rows of out start on 16-byte boundaries
 };
 
-__device__ __forceinline__ void int8_store(void* out, int64_t i, float v, int dtype) {
-  if (dtype == kInt8OutBf16)
-    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
-  else if (dtype == kInt8OutFp16)
-    static_cast<__half*>(out)[i] = __float2half_rn(v);
+// Outputs of 32 channels (one per lane) x M tokens: y[i] is row i's, the first `count` rows are
+// stored. Where rows start on 16-byte boundaries and all 32 channels exist, the block is turned
+// in shared memory (buf, 32 M elements) and stored in 16-byte pieces, else element by element.
+// (Two-byte stores alone, 64 bytes per instruction, took 6.8 us for a tile of 128 channels x
+// 256 tokens, longer than its MMAs at K = 1536.)
+template <typename T, int M>
+__device__ __forceinline__ void int8_store_rows_as(T* out, int64_t ldo, const float (&y)[M],
+                                                   int count, int channels, bool vec,
+                                                   uint8_t* buf, int lane) {
+  auto as_out = [](float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+    else return __float2bfloat16_rn(v);
+  };
+  if (vec && channels >= 32) {
+    constexpr int kPieces = 2 * sizeof(T);  // 16-byte pieces of a row
+    constexpr int kRows = 32 / kPieces;     // rows per store instruction
+    T* turn = reinterpret_cast<T*>(buf);
+    __syncwarp();  // the previous block is stored
+#pragma unroll
+    for (int i = 0; i < M; ++i) turn[32 * i + lane] = as_out(y[i]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < M; i += kRows) {
+      const int r = i + lane / kPieces;
+      if (r < count)
+        *reinterpret_cast<uint4*>(out + r * ldo + lane % kPieces * (32 / kPieces)) =
+            *reinterpret_cast<const uint4*>(buf + 16 * (kPieces * r + lane % kPieces));
+    }
+  } else if (lane < channels) {
+    out += lane;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      if (i < count) *out = as_out(y[i]);
+      out += ldo;
+    }
+  }
+}
+// row0: first token row; n0: the lanes' first channel.
+template <int M>
+__device__ __forceinline__ void int8_store_rows(const Int8GemmParams& p, int64_t row0, int n0,
+                                                const float (&y)[M], int count, uint8_t* buf,
+                                                int lane) {
+  const int64_t at = row0 * p.ldo + n0;
+  const int channels = p.n - n0;
+  const bool vec = p.out_vec != 0;
+  if (p.out_dtype == kInt8OutBf16)
+    int8_store_rows_as(static_cast<__nv_bfloat16*>(p.out) + at, p.ldo, y, count, channels, vec, buf,
+                       lane);
+  else if (p.out_dtype == kInt8OutFp16)
+    int8_store_rows_as(static_cast<__half*>(p.out) + at, p.ldo, y, count, channels, vec, buf, lane);
   else
-    static_cast<float*>(out)[i] = v;
+    int8_store_rows_as(static_cast<float*>(p.out) + at, p.ldo, y, count, channels, vec, buf, lane);
 }
 
 __device__ __forceinline__ float int8_silu_mul(float g, float u) {
@@ -108,6 +158,9 @@ struct Int8Tile {
   int expert, row, rows, nt;  // rows: valid token rows of the tile
 };
 
+// Tile `tile` of the launch. BALANCED: an expert's tiles have equal rows (a multiple of 32, at
+// most tile_rows), the last one the remainder.
+template <bool BALANCED>
 __device__ __forceinline__ Int8Tile int8_find_tile(int tile, int tile_rows, int n_tiles,
                                                    int num_experts, const int32_t* seg_row,
                                                    const int32_t* seg_cnt,
@@ -122,28 +175,31 @@ __device__ __forceinline__ Int8Tile int8_find_tile(int tile, int tile_rows, int 
   const int tiles_m = (cnt + tile_rows - 1) / tile_rows;
   const int local = tile - (seg_end[lo] - tiles_m * n_tiles);
   const int mt = local % tiles_m;
-  return {lo, seg_row[lo] + mt * tile_rows, min(tile_rows, cnt - mt * tile_rows), local / tiles_m};
+  const int rows = BALANCED ? ((cnt + tiles_m - 1) / tiles_m + 31) / 32 * 32 : tile_rows;
+  return {lo, seg_row[lo] + mt * rows, min(rows, cnt - mt * rows), local / tiles_m};
 }
 
 template <int TN, bool GATED>
 struct Int8Config {
   static constexpr int kSets = GATED ? 2 : 1;
+  static constexpr int kEpiWarps = TN >= 64 ? 8 : 4;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kWBytes = 128 * kInt8StageK;
   static constexpr int kXBytes = TN * kInt8StageK;
   static constexpr int kStageBytes = kSets * kWBytes + kXBytes;
-  static constexpr int kFixedBytes = 1024 + kInt8SegBytes + 512;
+  static constexpr int kTurnBytes = 16 * 128;  // a warp's block of 16 tokens x 32 channels
+  static constexpr int kFixedBytes = 1024 + kInt8SegBytes + kEpiWarps * kTurnBytes + 512;
   static constexpr int kFit = (232448 - kFixedBytes) / kStageBytes;
   static constexpr int kStages = kFit > 12 ? 12 : kFit;
   static constexpr int kSmemBytes = kFixedBytes + kStages * kStageBytes;
   static constexpr int kAccCols = TN * kSets;
   static constexpr int kTmemColumns = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
-  static constexpr uint32_t kIdesc = ptx::make_idesc_i8(128, TN);
   static_assert(kStages >= 3 && 8 * (2 * kStages + 5) + 16 <= 512, "shared memory layout");
   static_assert((kTmemColumns & (kTmemColumns - 1)) == 0 && kTmemColumns <= 512, "TMEM columns");
 };
 
 template <int TN, bool GATED>
-__global__ void __launch_bounds__(kNumThreads, 1)
+__global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
     nvfp4_int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                            const __grid_constant__ CUtensorMap map_b,
                            const __grid_constant__ CUtensorMap map_b2,
@@ -153,7 +209,8 @@ __global__ void __launch_bounds__(kNumThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  int32_t* seg_row = reinterpret_cast<int32_t*>(smem + kStages * Cfg::kStageBytes);
+  uint8_t* turn = smem + kStages * Cfg::kStageBytes;
+  int32_t* seg_row = reinterpret_cast<int32_t*>(turn + Cfg::kEpiWarps * Cfg::kTurnBytes);
   int32_t* seg_cnt = seg_row + kInt8MaxExperts;
   int32_t* seg_end = seg_cnt + kInt8MaxExperts;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(seg_end + kInt8MaxExperts);
@@ -173,7 +230,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(&accf_bar[a], 1);
-      ptx::mbar_init(&acce_bar[a], kEpilogueWarps);
+      ptx::mbar_init(&acce_bar[a], Cfg::kEpiWarps);
     }
     ptx::mbar_init(drain_bar, 1);
     *abort_flag = 0u;
@@ -206,7 +263,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       bool ok = true;
       for (int tile = first; ok && tile < total; tile += step) {
         const Int8Tile t =
-            int8_find_tile(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+            int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
         const int wrow = t.expert * p.n + t.nt * 128;
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&empty_bar[stage], phase ^ 1u, abort_flag, p.error_bits,
@@ -256,6 +313,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         acc_parity ^= 1u << acc;
         ptx::tcgen05_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * Cfg::kAccCols;
+        const Int8Tile t =
+            int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+        const uint32_t idesc = ptx::make_idesc_i8(128, (t.rows + 15) / 16 * 16);
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&full_bar[stage], phase, abort_flag, p.error_bits, kDevErrMmaTimeout)) {
             ok = false;
@@ -267,13 +327,13 @@ __global__ void __launch_bounds__(kNumThreads, 1)
           const uint64_t x_desc = ptx::make_sw128_kmajor_desc(sW + Cfg::kSets * Cfg::kWBytes);
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb)
-            ptx::mma_i8(d_tmem, w_desc + 2 * kb, x_desc + 2 * kb, Cfg::kIdesc,
+            ptx::mma_i8(d_tmem, w_desc + 2 * kb, x_desc + 2 * kb, idesc,
                         (kt | kb) != 0 ? 1u : 0u);
           if (GATED) {
             const uint64_t w2_desc = ptx::make_sw128_kmajor_desc(sW + Cfg::kWBytes);
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
-              ptx::mma_i8(d_tmem + TN, w2_desc + 2 * kb, x_desc + 2 * kb, Cfg::kIdesc,
+              ptx::mma_i8(d_tmem + TN, w2_desc + 2 * kb, x_desc + 2 * kb, idesc,
                           (kt | kb) != 0 ? 1u : 0u);
           }
           ptx::tcgen05_commit(&empty_bar[stage]);
@@ -296,17 +356,32 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
+    // This warp's tokens of a tile: all of them, or one half.
+    constexpr int kToks = TN / (Cfg::kEpiWarps / 4);
+    const int tok0 = (warp - kEpilogueWarp0) / 4 * kToks;
     uint32_t full_parity = 0;
     uint32_t local = 0;
     for (int tile = first; tile < total; tile += step, ++local) {
       const Int8Tile t =
-          int8_find_tile(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+          int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
       const int n = t.nt * 128 + 32 * quarter + lane;
       const bool in = n < p.n;
       const int64_t chan = static_cast<int64_t>(t.expert) * p.n + n;
       const float bs = in ? __ldg(p.b_scale + chan) : 0.0f;
       const float bs2 = GATED && in ? __ldg(p.b2_scale + chan) : 0.0f;
       const float bias = !GATED && in && p.bias != nullptr ? __ldg(p.bias + n) : 0.0f;
+      // Token scales, one per lane, handed out by shuffles.
+      float as[(kToks + 31) / 32];
+#pragma unroll
+      for (int i = 0; i < (kToks + 31) / 32; ++i) {
+        const int tok = tok0 + 32 * i + lane;
+        as[i] = tok < t.rows ? __ldg(p.a_scale + t.row + tok) : 0.0f;
+      }
+      auto value = [&](int32_t g, int32_t w, float a) {
+        const float y = __fmul_rn(__fmul_rn(__int2float_rn(g), a), bs);
+        return GATED ? int8_silu_mul(y, __fmul_rn(__fmul_rn(__int2float_rn(w), a), bs2))
+                     : __fadd_rn(y, bias);
+      };
       const int acc = static_cast<int>(local & 1u);
       if (!warp_wait_phase(&accf_bar[acc], (full_parity >> acc) & 1u, abort_flag, p.error_bits,
                            kDevErrEpilogueTimeout, lane))
@@ -314,28 +389,27 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       full_parity ^= 1u << acc;
       ptx::tcgen05_fence_after_sync();
       const uint32_t t_acc =
-          tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) + acc * Cfg::kAccCols;
-      for (int c = 0; c < t.rows; c += 16) {
-        uint32_t v[16], u[16];
+          tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) + acc * Cfg::kAccCols + tok0;
+      const int toks = min(kToks, t.rows - tok0);
+      auto load16 = [&](int c, uint32_t(&v)[16], uint32_t(&u)[16]) {
         ptx::tmem_ld_32x32b_x16(t_acc + c, v);
         if (GATED) ptx::tmem_ld_32x32b_x16(t_acc + TN + c, u);
         ptx::tmem_ld_wait();
         ptx::reg_fence(v);
         if (GATED) ptx::reg_fence(u);
+      };
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (c + i >= t.rows) break;  // uniform over the warp
-          const int64_t row = static_cast<int64_t>(t.row) + c + i;
-          const float as = __ldg(p.a_scale + row);
-          float y = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(v[i])), as), bs);
-          if (GATED) {
-            const float w = __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(u[i])), as), bs2);
-            y = int8_silu_mul(y, w);
-          } else {
-            y = __fadd_rn(y, bias);
-          }
-          if (in) int8_store(p.out, row * p.ldo + n, y, p.out_dtype);
-        }
+      for (int c = 0; c < kToks; c += 16) {
+        if (c >= toks) break;  // uniform over the warp
+        uint32_t v[16], u[16];
+        load16(c, v, u);
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          y[i] = value(static_cast<int32_t>(v[i]), GATED ? static_cast<int32_t>(u[i]) : 0,
+                       __shfl_sync(0xffffffffu, as[c / 32], (c + i) & 31));
+        int8_store_rows(p, static_cast<int64_t>(t.row) + tok0 + c, n - lane, y, toks - c,
+                        turn + (warp - kEpilogueWarp0) * Cfg::kTurnBytes, lane);
       }
       ptx::tcgen05_fence_before_sync();
       __syncwarp();

@@ -1,0 +1,170 @@
+// The int8 product for a few tokens and few weight tiles: sums of byte products on the CUDA
+// cores (dp4a), one warp per two channels (one: 7.4 us at N 7168, K 2048, two: 4.9, four: 5.6).
+//
+// A tensor-core tile takes 128 weight rows at 64 bytes per cycle at best, so a weight matrix of
+// fewer tiles than SMs (N = 4096: 32) cannot be streamed at the memory's rate (N 4096, K 7168,
+// one token: 11.4 us; here 8.6, 3.4 TB/s, a launch that does nothing takes 2.6). Here every warp
+// of the GPU streams rows of its own: a lane loads 16 bytes of K of each row, 8 loads in
+// flight, multiplies them with the codes of up to TB tokens, which all warps of an SM share in
+// L1, and the warp adds up.
+// Segments of more than TB rows are taken in several passes over the (cached) weights.
+#pragma once
+
+#include "int8_gemm_kernel.cuh"
+
+namespace nvfp4 {
+
+constexpr int kInt8GemvThreads = 256;
+constexpr int kInt8GemvRows = 2;  // channels of a warp
+
+// 16 bytes at byte c of a row of k bytes, zeros past its end.
+template <bool STREAM>
+__device__ __forceinline__ uint4 int8_load16(const uint8_t* __restrict__ row, int c, int k) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (c + 16 <= k) {
+    if (STREAM)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "l"(row + c));
+    else
+      v = __ldg(reinterpret_cast<const uint4*>(row + c));
+  } else if (c < k) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < k) w[i / 4] |= static_cast<uint32_t>(__ldg(row + c + i)) << (8 * (i % 4));
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+
+__device__ __forceinline__ int32_t int8_dot16(const uint4& a, const uint4& b, int32_t acc) {
+  acc = __dp4a(static_cast<int>(a.x), static_cast<int>(b.x), acc);
+  acc = __dp4a(static_cast<int>(a.y), static_cast<int>(b.y), acc);
+  acc = __dp4a(static_cast<int>(a.z), static_cast<int>(b.z), acc);
+  return __dp4a(static_cast<int>(a.w), static_cast<int>(b.w), acc);
+}
+
+struct Int8GemvParams {
+  Int8GemmParams p;
+  const uint8_t* a;
+  const uint8_t* b;
+  const uint8_t* b2;
+  int64_t lda, ldb;
+  int32_t k;
+};
+
+template <int TB, bool GATED>
+__global__ void __launch_bounds__(kInt8GemvThreads)
+    nvfp4_int8_gemv_kernel(const __grid_constant__ Int8GemvParams q) {
+  constexpr int R = kInt8GemvRows;
+  constexpr int kRows = R * (GATED ? 2 : 1);  // weight rows of a warp
+  constexpr int kAhead = 8 / kRows;           // 16-byte loads in flight per row
+  const Int8GemmParams& p = q.p;
+  __shared__ int32_t used[kInt8MaxExperts];  // experts with rows
+  __shared__ int32_t num_used;
+  const int lane = threadIdx.x & 31;
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int base = 0; base < p.num_experts; base += 32) {
+      const int e = base + lane;
+      bool has = false;
+      if (e < p.num_experts) {
+        int32_t off = 0, cnt = p.rows;
+        if (p.seg_offsets != nullptr) {
+          off = __ldg(p.seg_offsets + e);
+          cnt = __ldg(p.seg_counts + e);
+        }
+        if (cnt < 0 || off < 0 || static_cast<int64_t>(off) + cnt > p.rows)
+          atomicOr(p.error_bits, kDevErrBadSegment);
+        else
+          has = cnt > 0;
+      }
+      const uint32_t mask = __ballot_sync(0xffffffffu, has);
+      if (has) used[n + __popc(mask & ((1u << lane) - 1u))] = e;
+      n += __popc(mask);
+    }
+    if (lane == 0) num_used = n;
+  }
+  __syncthreads();
+  const int groups = (p.n + R - 1) / R;
+  const int64_t units = static_cast<int64_t>(num_used) * groups;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kInt8GemvThreads / 32);
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * (kInt8GemvThreads / 32) +
+                      (threadIdx.x >> 5);
+       unit < units; unit += step) {
+    const int e = used[unit / groups];
+    const int n0 = static_cast<int>(unit % groups) * R;
+    const int32_t row0 = p.seg_offsets != nullptr ? __ldg(p.seg_offsets + e) : 0;
+    const int32_t cnt = p.seg_counts != nullptr ? __ldg(p.seg_counts + e) : p.rows;
+    const uint8_t* w[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t row = static_cast<int64_t>(e) * p.n + min(n0 + i % R, p.n - 1);
+      w[i] = (i < R ? q.b : q.b2) + row * q.ldb;
+    }
+    for (int t0 = 0; t0 < cnt; t0 += TB) {
+      const uint8_t* x[TB];
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+        x[t] = q.a + (static_cast<int64_t>(row0) + min(t0 + t, cnt - 1)) * q.lda;
+      int32_t acc[kRows][TB];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) acc[i][t] = 0;
+      for (int c0 = 16 * lane; c0 < q.k; c0 += 512 * kAhead) {
+        uint4 wv[kRows][kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) wv[i][u] = int8_load16<true>(w[i], c0 + 512 * u, q.k);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+          for (int t = 0; t < TB; ++t) {
+            const uint4 xv = int8_load16<false>(x[t], c0 + 512 * u, q.k);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) acc[i][t] = int8_dot16(wv[i][u], xv, acc[i][t]);
+          }
+      }
+      // Lane r + R t finishes channel n0 + r of token t0 + t.
+      int32_t g = 0, h = 0;
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int32_t s = __reduce_add_sync(0xffffffffu, acc[r][t]);
+          if (lane == r + R * t) g = s;
+          if (GATED) {
+            const int32_t s2 = __reduce_add_sync(0xffffffffu, acc[kRows - R + r][t]);
+            if (lane == r + R * t) h = s2;
+          }
+        }
+      const int n = n0 + lane % R;
+      const int tok = t0 + lane / R;
+      if (lane < R * TB && n < p.n && tok < cnt) {
+        const int64_t row = static_cast<int64_t>(row0) + tok;
+        const int64_t chan = static_cast<int64_t>(e) * p.n + n;
+        const float as = __ldg(p.a_scale + row);
+        float y = __fmul_rn(__fmul_rn(__int2float_rn(g), as), __ldg(p.b_scale + chan));
+        if (GATED)
+          y = int8_silu_mul(y, __fmul_rn(__fmul_rn(__int2float_rn(h), as),
+                                         __ldg(p.b2_scale + chan)));
+        else
+          y = __fadd_rn(y, p.bias != nullptr ? __ldg(p.bias + n) : 0.0f);
+        const int64_t at = row * p.ldo + n;
+        if (p.out_dtype == kInt8OutBf16)
+          static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+        else if (p.out_dtype == kInt8OutFp16)
+          static_cast<__half*>(p.out)[at] = __float2half_rn(y);
+        else
+          static_cast<float*>(p.out)[at] = y;
+      }
+    }
+  }
+}
+
+}  // namespace nvfp4

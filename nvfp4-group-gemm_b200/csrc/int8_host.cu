@@ -9,6 +9,8 @@
 #include "../../include/nvfp4_group_gemm.h"
 #include "host_common.cuh"
 #include "int8_gemm_kernel.cuh"
+#include "int8_gemm_pair_kernel.cuh"
+#include "int8_gemv_kernel.cuh"
 #include "int8_quantize_kernel.cuh"
 
 namespace nvfp4 {
@@ -33,6 +35,18 @@ cudaError_t allow_smem() {
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Int8Config<TN, GATED>::kSmemBytes);
 }
+template <bool GATED>
+cudaError_t allow_smem_all() {
+  cudaError_t e = allow_smem<16, GATED>();
+  if (e == cudaSuccess) e = allow_smem<32, GATED>();
+  if (e == cudaSuccess) e = allow_smem<64, GATED>();
+  if (e == cudaSuccess) e = allow_smem<128, GATED>();
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(nvfp4_int8_gemm_pair_kernel<GATED>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Int8PairConfig<GATED>::kSmemBytes);
+  return e;
+}
 
 // Once per device. The look-up may load the module, which a stream capture under way on this
 // thread would otherwise forbid.
@@ -42,14 +56,8 @@ void init_int8_device(Int8Device& d) {
   void* p = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&p, g_int8_error_bits);
   d.error_bits = static_cast<uint32_t*>(p);
-  if (e == cudaSuccess) e = allow_smem<16, false>();
-  if (e == cudaSuccess) e = allow_smem<32, false>();
-  if (e == cudaSuccess) e = allow_smem<64, false>();
-  if (e == cudaSuccess) e = allow_smem<128, false>();
-  if (e == cudaSuccess) e = allow_smem<16, true>();
-  if (e == cudaSuccess) e = allow_smem<32, true>();
-  if (e == cudaSuccess) e = allow_smem<64, true>();
-  if (e == cudaSuccess) e = allow_smem<128, true>();
+  if (e == cudaSuccess) e = allow_smem_all<false>();
+  if (e == cudaSuccess) e = allow_smem_all<true>();
   d.status = e;
   cudaThreadExchangeStreamCaptureMode(&mode);
 }
@@ -79,32 +87,108 @@ bool int8_map(CUtensorMap* m, const void* addr, int64_t rows, int k, int64_t ld,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
-template <int TN, bool GATED>
-int launch_int8(const nvfp4_int8_product* g, Int8GemmParams& p, int num_sms, cudaStream_t s) {
-  CUtensorMap ma, mb, mb2;
+// Tensor maps of a product: tokens in boxes of `x_box` rows, weights in boxes of `w_box`.
+struct Int8Maps {
+  CUtensorMap a, b, b2;
+};
+bool int8_maps(const nvfp4_int8_product* g, int x_box, int w_box, Int8Maps* m) {
   const int64_t wrows = static_cast<int64_t>(g->num_experts) * g->n;
-  if (!int8_map(&ma, g->a, g->rows, g->k, g->lda, TN) ||
-      !int8_map(&mb, g->b, wrows, g->k, g->ldb, 128) ||
-      !int8_map(&mb2, GATED ? g->b2 : g->b, wrows, g->k, g->ldb, 128))
-    return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
-  const int64_t n_tiles = (g->n + 127) / 128;
-  // The most tiles any segments can need: every row tile full, and one ragged tile each.
-  const int64_t tiles = ((g->rows + TN - 1) / TN + (g->num_experts - 1)) * n_tiles;
+  if (!int8_map(&m->a, g->a, g->rows, g->k, g->lda, x_box) ||
+      !int8_map(&m->b, g->b, wrows, g->k, g->ldb, w_box))
+    return false;
+  if (g->b2 == nullptr) {
+    m->b2 = m->b;
+    return true;
+  }
+  return int8_map(&m->b2, g->b2, wrows, g->k, g->ldb, w_box);
+}
+
+// The most tiles any segments can need: every row tile full, and one ragged tile each.
+int64_t int8_max_tiles(const nvfp4_int8_product* g, int tile_rows, int tile_n) {
+  return ((g->rows + tile_rows - 1) / tile_rows + (g->num_experts - 1)) *
+         ((g->n + tile_n - 1) / tile_n);
+}
+
+template <int TN, bool GATED>
+int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sms, cudaStream_t s) {
+  using Cfg = Int8Config<TN, GATED>;
+  Int8Maps m;
+  if (!int8_maps(g, TN, 128, &m)) return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
+  const int64_t tiles = int8_max_tiles(g, TN, 128);
   if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
-  const int64_t grid = std::min<int64_t>(tiles, num_sms);
   const cudaError_t e =
-      launch_dependent(&nvfp4_int8_gemm_kernel<TN, GATED>, grid, kNumThreads,
-                       Int8Config<TN, GATED>::kSmemBytes, s, ma, mb, mb2, p);
+      launch_dependent(&nvfp4_int8_gemm_kernel<TN, GATED>, std::min<int64_t>(tiles, num_sms),
+                       Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.b, m.b2, p);
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
+}
+
+template <int TB, bool GATED>
+int launch_int8_gemv(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sms,
+                     cudaStream_t s) {
+  Int8GemvParams q = {};
+  q.p = p;
+  q.a = static_cast<const uint8_t*>(g->a);
+  q.b = static_cast<const uint8_t*>(g->b);
+  q.b2 = static_cast<const uint8_t*>(g->b2);
+  q.lda = g->lda;
+  q.ldb = g->ldb;
+  q.k = g->k;
+  const int64_t warps =
+      (static_cast<int64_t>(g->n) + kInt8GemvRows - 1) / kInt8GemvRows * g->num_experts;
+  const int64_t blocks = (warps + kInt8GemvThreads / 32 - 1) / (kInt8GemvThreads / 32);
+  const cudaError_t e =
+      launch_dependent(&nvfp4_int8_gemv_kernel<TB, GATED>,
+                       std::min<int64_t>(blocks, num_sms * 4), kInt8GemvThreads, 0, s, q);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
 template <bool GATED>
-int choose_int8(const nvfp4_int8_product* g, Int8GemmParams& p, int num_sms, cudaStream_t s) {
+int launch_int8_pair(const nvfp4_int8_product* g, const Int8GemmParams& p, int clusters,
+                     cudaStream_t s) {
+  using Cfg = Int8PairConfig<GATED>;
+  Int8Maps m;
+  if (!int8_maps(g, kInt8PairTokens / 2, Cfg::kWBox, &m))
+    return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
+  const int64_t tiles = int8_max_tiles(g, kInt8PairTokens, Cfg::kOutN);
+  if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
+  const cudaError_t e =
+      launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED>, std::min<int64_t>(tiles, clusters) * 2,
+                      2, kInt8PairThreads, Cfg::kSmemBytes, s, m.a, m.b, m.b2, p);
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
+}
+
+// Kernel and tile of a product, from the rows that the segments are expected to hold. Times in us
+// on a B200, one launch of many, weights not in L2.
+//
+// Few tiles (fewer 128-channel tiles than SMs): a launch takes as long as one CTA's K loop, so
+// the smallest token tile that still runs in one wave is taken. Dense, N 4096, K 7168: 256 rows
+// 13.2 with tiles of 64, 16.5 with 128; 512 rows 16.9 with 128, 21.4 with 64. With one or two
+// rows per expert the weights are streamed by all SMs without tiles (int8_gemv_kernel.cuh):
+// one row 8.6 against 11.4, two rows 11.1 against 11.5; at four rows it loses (17 against 11.5).
+//
+// Many tiles: bound by the weights' bytes while an expert's rows fit one tile, so tiles are
+// chosen to hold them with a quarter to spare (64 experts of 64 +- 8 rows, N 4096, K 1536:
+// 70.5 with 128 tokens, 75.6 with 64); above 80 rows the MMAs decide and CTA pairs are faster
+// (128 rows: 81 against 97 with 128-token tiles, gated N 1536, K 4096 155 against 159;
+// 64 rows: 141 against 137).
+template <bool GATED>
+int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const DeviceState& ds,
+                cudaStream_t s) {
+  const int num_sms = ds.num_sms;
   const int64_t expected = g->expected_rows > 0 ? std::min(g->expected_rows, g->rows) : g->rows;
-  const int64_t per_expert = (expected + g->num_experts - 1) / g->num_experts;
-  if (per_expert <= 16) return launch_int8<16, GATED>(g, p, num_sms, s);
-  if (per_expert <= 32) return launch_int8<32, GATED>(g, p, num_sms, s);
-  if (per_expert <= 64) return launch_int8<64, GATED>(g, p, num_sms, s);
+  const int64_t active = std::min<int64_t>(g->num_experts, expected);  // experts with rows
+  const int64_t rows = (expected + active - 1) / active;
+  const int64_t n_tiles = (g->n + 127) / 128;
+  if (rows <= 2 && active * n_tiles < num_sms)
+    return rows == 1 ? launch_int8_gemv<1, GATED>(g, p, num_sms, s)
+                     : launch_int8_gemv<2, GATED>(g, p, num_sms, s);
+  auto one_wave = [&](int tn) { return active * ((rows + tn - 1) / tn) * n_tiles <= num_sms; };
+  const bool many = !one_wave(128);
+  if (many && rows > 80) return launch_int8_pair<GATED>(g, p, ds.pair_clusters, s);
+  auto fits = [&](int tn) { return many ? 4 * tn >= 5 * rows : one_wave(tn); };
+  if (fits(16)) return launch_int8<16, GATED>(g, p, num_sms, s);
+  if (fits(32)) return launch_int8<32, GATED>(g, p, num_sms, s);
+  if (fits(64)) return launch_int8<64, GATED>(g, p, num_sms, s);
   return launch_int8<128, GATED>(g, p, num_sms, s);
 }
 
@@ -241,8 +325,9 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
   p.out_dtype = g->out_dtype == NVFP4_DTYPE_BF16   ? kInt8OutBf16
                 : g->out_dtype == NVFP4_DTYPE_FP16 ? kInt8OutFp16
                                                    : kInt8OutFp32;
+  p.out_vec = aligned16(g->out) && g->ldo * (p.out_dtype == kInt8OutFp32 ? 4 : 2) % 16 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return gated ? choose_int8<true>(g, p, ds->num_sms, s) : choose_int8<false>(g, p, ds->num_sms, s);
+  return gated ? choose_int8<true>(g, p, *ds, s) : choose_int8<false>(g, p, *ds, s);
 }
 
 NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits) {

@@ -23,25 +23,28 @@ _IN_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F
 _OUT_DTYPES = {**_IN_DTYPES, torch.float32: _native.DTYPE_FP32}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _launch_on(tensors, stream: torch.cuda.Stream | None) -> tuple:
-    """``(stream, context)`` of a call on ``tensors`` (the first gives the device; the others must
-    be on it). The context makes device and stream current, so that what is allocated inside
-    belongs to the stream. Tensors used on another stream than the current one are recorded
-    there, so that freeing them early does not hand their memory out while the call runs."""
-    dev = tensors[0].device
+    """``(raw stream, context)`` of a call on ``tensors`` (None entries left out; the first gives
+    the device, the others must be on it). The context makes device and stream current, so that
+    what is allocated inside belongs to the stream. Tensors used on another stream than the
+    current one are recorded there, so that freeing them early does not hand their memory out
+    while the call runs."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != dev):
+        if t is not None and t.get_device() != index or index < 0:
             raise ValueError("all tensors must be CUDA tensors on one device")
-    current = torch.cuda.current_stream(dev)
-    if stream is None or stream == current:
-        on_dev = torch.cuda.current_device() == dev.index
-        return current, contextlib.nullcontext() if on_dev else torch.cuda.device(dev)
-    if stream.device != dev:
-        raise ValueError(f"stream is on {stream.device}, the tensors are on {dev}")
+    raw = torch._C._cuda_getCurrentRawStream(index)
+    if stream is None or (stream.cuda_stream == raw and stream.device.index == index):
+        return raw, _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+    if stream.device.index != index:
+        raise ValueError(f"stream is on {stream.device}, the tensors are on cuda:{index}")
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
-    return stream, torch.cuda.stream(stream)
+    return stream.cuda_stream, torch.cuda.stream(stream)
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -68,13 +71,15 @@ def _codes_stride(t: torch.Tensor, name: str) -> int:
     """Bytes between the rows of an int8 code matrix [rows, k] (checked)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int8:
         raise ValueError(f"{name} must be a CUDA int8 tensor")
-    if t.dim() != 2 or t.shape[1] < 1 or not _unit_inner(t):
-        raise ValueError(f"{name} must be 2-D with unit stride along the last dimension")
-    if t.shape[0] <= 1:
-        ld = -(-int(t.shape[1]) // 16) * 16
-    else:
-        ld = int(t.stride(0))
-    if ld % 16 or ld < t.shape[1] or t.data_ptr() % 16:
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if cols < 1 or (inner != 1 and cols != 1):
+        raise ValueError(f"{name} must have unit stride along the last dimension")
+    if rows <= 1:
+        ld = (cols + 15) // 16 * 16
+    if ld % 16 or ld < cols or t.data_ptr() % 16:
         raise ValueError(f"rows of {name} must start on 16-byte boundaries "
                          "(quantize_int8 allocates them so)")
     return ld
@@ -82,7 +87,7 @@ def _codes_stride(t: torch.Tensor, name: str) -> int:
 
 def _check_scale(t: torch.Tensor, shape: tuple, name: str) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or \
-            tuple(t.shape) != shape or not t.is_contiguous():
+            t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous CUDA float32 tensor of shape {list(shape)}")
 
 
@@ -128,7 +133,7 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor | None = None,
         _native.check(lib.nvfp4_quantize_int8(
             x.data_ptr(), rows, cols, _row_stride(x), _IN_DTYPES[x.dtype],
             row_mask.data_ptr() if row_mask is not None else None, codes.data_ptr(),
-            _codes_stride(codes, "codes"), scales.data_ptr(), s.cuda_stream), lib)
+            _codes_stride(codes, "codes"), scales.data_ptr(), s), lib)
     return codes, scales
 
 
@@ -168,7 +173,7 @@ def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, n, k, ex
     p.rows, p.n, p.k, p.num_experts = int(a.shape[0]), n, k, experts
     p.expected_rows = expected_rows
     lib = _native.load_library()
-    _native.check(lib.nvfp4_int8_gemm(ctypes.byref(p), stream.cuda_stream), lib)
+    _native.check(lib.nvfp4_int8_gemm(ctypes.byref(p), stream), lib)
 
 
 def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,

@@ -165,7 +165,7 @@ def dispatch_int8(x: torch.Tensor, routing: Routing, codes: torch.Tensor | None 
         _native.check(lib.nvfp4_moe_dispatch_int8(
             x.data_ptr(), routing.tokens, cols, _row_stride(x), _DTYPES[x.dtype], dest.data_ptr(),
             routing.topk, rows, codes.data_ptr(), _codes_stride(codes, "codes"),
-            scales.data_ptr(), s.cuda_stream), lib)
+            scales.data_ptr(), s), lib)
     return codes, scales
 
 

@@ -5,8 +5,8 @@
     ...                                          # the experts
     out = combine_tokens(rows, r, topk_weights)  # [tokens, H]
 
-bf16, fp16 and fp32, any width and row stride, differentiable (first order) in ``x``, the rows
-and the weights. Sums are fp32 in slot order, rounded once: results do not depend on timing.
+bf16, fp16 and fp32, any width and row stride, differentiable in ``x``, the rows and the
+weights (with weights: once). Sums are fp32 in slot order, rounded once: results do not depend on timing.
 The ``*_backward`` functions are the gradients by themselves, for training loops that do not go
 through autograd. The reference has no counterpart.
 """
@@ -33,8 +33,8 @@ def _check_routing(routing) -> tuple:
 def _check_rows(t: torch.Tensor, rows: int, name: str, cols: int | None = None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _OUT_DTYPES:
         raise ValueError(f"{name} must be a CUDA bf16, fp16 or fp32 tensor")
-    if t.dim() != 2 or int(t.shape[0]) != rows or t.shape[1] < 1 or \
-            (cols is not None and int(t.shape[1]) != cols):
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or \
+            (cols is not None and t.shape[1] != cols):
         want = f"[{rows}, {'cols' if cols is None else cols}]"
         raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
 
@@ -44,6 +44,12 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     if not _unit_inner(t) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         return t.contiguous()
     return t
+
+
+def _fp32(weights):
+    if weights is None or (weights.dtype == torch.float32 and weights.is_contiguous()):
+        return weights
+    return weights.to(torch.float32).contiguous()
 
 
 def _ptr(t):
@@ -61,7 +67,7 @@ def _dispatch(x, routing, stream):
         lib = _native.load_library()
         _native.check(lib.nvfp4_moe_dispatch_tokens(
             x.data_ptr(), _row_stride(x), _OUT_DTYPES[x.dtype], dest.data_ptr(), src.data_ptr(),
-            tokens, topk, cols, rows, y.data_ptr(), cols, s.cuda_stream), lib)
+            tokens, topk, cols, rows, y.data_ptr(), cols, s), lib)
     return y
 
 
@@ -78,13 +84,13 @@ def _combine(y, routing, weights, stream):
     s, where = _launch_on((y, dest, weights), stream)
     with where:
         y = _rows_of(y)
-        w = weights.to(torch.float32).contiguous() if weights is not None else None
+        w = _fp32(weights)
         cols = int(y.shape[1])
         out = torch.empty((tokens, cols), dtype=y.dtype, device=y.device)
         lib = _native.load_library()
         _native.check(lib.nvfp4_moe_combine_tokens(
             y.data_ptr(), _row_stride(y), _OUT_DTYPES[y.dtype], dest.data_ptr(), _ptr(w), tokens,
-            topk, cols, rows, out.data_ptr(), cols, s.cuda_stream), lib)
+            topk, cols, rows, out.data_ptr(), cols, s), lib)
     return out
 
 
@@ -120,7 +126,7 @@ def combine_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor | None, rout
     with where:
         g = _rows_of(grad_out)
         used_y = _rows_of(used_y) if want_weights else None
-        w = weights.to(torch.float32).contiguous() if weights is not None else None
+        w = _fp32(weights)
         dev = g.device
         gy = torch.empty((rows, cols), dtype=g.dtype, device=dev) if want_y else None
         gw = torch.empty((tokens, topk), dtype=torch.float32, device=dev) if want_weights else None
@@ -128,7 +134,7 @@ def combine_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor | None, rout
         _native.check(lib.nvfp4_moe_combine_tokens_backward(
             g.data_ptr(), _row_stride(g), _ptr(used_y), _row_stride(used_y) if want_weights else 0,
             _OUT_DTYPES[g.dtype], dest.data_ptr(), src.data_ptr(), _ptr(w), tokens, topk, cols, rows,
-            _ptr(gy), cols, _ptr(gw), s.cuda_stream), lib)
+            _ptr(gy), cols, _ptr(gw), s), lib)
     return gy, gw
 
 
@@ -148,10 +154,19 @@ class _DispatchTokens(torch.autograd.Function):
         return _dispatch(x, routing, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
         ctx.routing.dest, ctx.routing.src_rows = ctx.saved_tensors
-        return dispatch_tokens_backward(grad_y, ctx.routing), None
+        if torch.is_grad_enabled():  # the gradient of the gradient: the same two operators again
+            return combine_tokens(grad_y, ctx.routing), None
+        return _combine(grad_y, ctx.routing, None, None), None
+
+
+def _combine_gradients(ctx, grad_out):
+    dest, src, weights, y = ctx.saved_tensors
+    ctx.routing.dest, ctx.routing.src_rows = dest, src
+    gy, gw = combine_tokens_backward(grad_out, y, ctx.routing, weights,
+                                     want_y=ctx.needs_input_grad[0], want_weights=y is not None)
+    return gy, gw.to(weights.dtype) if gw is not None else None, None
 
 
 class _CombineTokens(torch.autograd.Function):
@@ -163,13 +178,14 @@ class _CombineTokens(torch.autograd.Function):
         return _combine(y, routing, weights, None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        dest, src, weights, y = ctx.saved_tensors
-        ctx.routing.dest, ctx.routing.src_rows = dest, src
-        gy, gw = combine_tokens_backward(grad_out, y, ctx.routing, weights,
-                                         want_y=ctx.needs_input_grad[0], want_weights=y is not None)
-        return gy, gw.to(weights.dtype) if gw is not None else None, None
+        if torch.is_grad_enabled():
+            if ctx.saved_tensors[2] is None:
+                dest, src = ctx.saved_tensors[:2]
+                ctx.routing.dest, ctx.routing.src_rows = dest, src
+                return dispatch_tokens(grad_out, ctx.routing), None, None
+            return once_differentiable(_combine_gradients)(ctx, grad_out)
+        return _combine_gradients(ctx, grad_out)
 
 
 def dispatch_tokens(x: torch.Tensor, routing,

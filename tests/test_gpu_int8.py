@@ -136,6 +136,18 @@ def test_product_larger(pkg, m, n, k):
     _check_product(pkg.int8_gemm(a, sa, b, sb), a, sa, b, sb)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(2, 300, 1000), (1, 4099, 17), (1300, 2050, 520),
+                                   (1100, 2304, 300), (3000, 1111, 257), (700, 2048, 1024)])
+def test_product_of_every_kernel(pkg, m, n, k, dtype):
+    """Sizes at which one or two rows, few tiles, many tiles and CTA pairs are chosen."""
+    a, b = _codes(m, k, 21), _codes(n, k, 22)
+    sa, sb = _scale(m, 23, 0.01), _scale(n, 24, 0.002)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(5)).cuda()
+    _check_product(pkg.int8_gemm(a, sa, b, sb, bias=bias, out_dtype=dtype), a, sa, b, sb, bias)
+    assert pkg.check_int8_errors() == 0
+
+
 def test_product_sums_are_exact_at_the_largest_k(pkg):
     """Sums next to the edge of int32, and codes of -128."""
     k = pkg._native.INT8_MAX_K
@@ -228,6 +240,21 @@ def test_segments_of_every_tile_shape(pkg, per, gated, dtype):
     offs = np.concatenate([[0], np.cumsum([(c + 127) // 128 * 128 for c in cnts])])[:E].tolist()
     rows = offs[-1] + 128
     _segments_case(pkg, offs, cnts, rows, 301, 333, gated, dtype, per * E, seed=per)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("per,n", [(1, 300), (2, 333), (8, 4000), (20, 2000), (40, 5000),
+                                   (50, 2500), (60, 5000), (130, 1300), (130, 3000), (260, 3008),
+                                   (520, 2048)])
+def test_segments_of_every_kernel(pkg, per, n, gated, dtype):
+    """Rows per expert and widths at which each kernel and token tile is chosen; the real counts
+    differ from the estimate, some far above it."""
+    E = 5
+    cnts = [per, 0, per + 9, max(per - 2, 0), 2 * per]
+    offs = np.concatenate([[0], np.cumsum([c + 3 for c in cnts])])[:E].tolist()
+    _segments_case(pkg, offs, cnts, offs[-1] + cnts[-1] + 2, n, 180, gated, dtype, per * E, seed=per)
+    assert pkg.check_int8_errors() == 0
 
 
 def test_many_experts(pkg):

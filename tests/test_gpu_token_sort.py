@@ -214,3 +214,24 @@ def test_autograd_captured_in_a_graph(pkg):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_second_gradients(pkg):
+    """Without weights both operators are linear and differentiable again; with weights the
+    second gradient is refused."""
+    r = pkg.moe.route(_ids(12, 2, 4, 5), 4)
+    x = _randn((12, 24), 1, torch.float32).requires_grad_(True)
+    y = pkg.moe.dispatch_tokens(x, r)
+    gy = _randn(tuple(y.shape), 2, torch.float32).requires_grad_(True)
+    (gx,) = torch.autograd.grad(y, x, gy, create_graph=True)
+    c = _randn((12, 24), 3, torch.float32)
+    (ggy,) = torch.autograd.grad(gx, gy, c)
+    assert torch.equal(ggy, pkg.moe.dispatch_tokens(c, r))
+    out = pkg.moe.combine_tokens(gy, r)
+    (g1,) = torch.autograd.grad(out, gy, c.requires_grad_(True), create_graph=True)
+    (g2,) = torch.autograd.grad(g1, c, gy.detach())
+    assert torch.equal(g2, out)
+    w = torch.rand((12, 2), device="cuda").requires_grad_(True)
+    (g3,) = torch.autograd.grad(pkg.moe.combine_tokens(gy, r, w), gy, c, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g3.sum().backward()
