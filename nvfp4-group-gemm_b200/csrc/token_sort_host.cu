@@ -2,6 +2,8 @@
 // nvfp4_moe_combine_tokens, nvfp4_moe_combine_tokens_backward).
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/nvfp4_group_gemm.h"
 #include "host_common.cuh"
 #include "token_sort_kernels.cuh"
@@ -33,21 +35,26 @@ int check_sizes(int tokens, int topk, int cols, int64_t rows, int dtype, const v
 enum class SortOp { kDispatch, kCombine, kBackward };
 
 template <typename T, int VEC>
-cudaError_t launch(SortOp op, const TokenSortParams& p, cudaStream_t s) {
-  const int64_t row_groups = (static_cast<int64_t>(p.rows) + 31) / 32;
-  const int warps = kSortThreads / 32;
+cudaError_t launch(SortOp op, const TokenSortParams& p, int num_sms, cudaStream_t s) {
+  const int64_t groups =
+      p.out != nullptr ? (static_cast<int64_t>(p.rows) + kPadRows - 1) / kPadRows : 0;
   if (op == SortOp::kBackward)
-    return launch_dependent(&nvfp4_combine_tokens_backward_kernel<T, VEC>,
-                            p.tokens + (p.out != nullptr ? row_groups : 0), kSortThreads, 0, s, p);
+    return launch_dependent(&nvfp4_combine_tokens_backward_kernel<T, VEC>, groups + p.tokens,
+                            kTokenThreads, 0, s, p);
   if (op == SortOp::kDispatch) {
+    const int warps = kSortThreads / 32;
     const int64_t chunks = (p.cols + 32 * VEC * kSortPieces - 1) / (32 * VEC * kSortPieces);
     return launch_dependent(&nvfp4_dispatch_tokens_kernel<T, VEC>,
-                            ((p.tokens + row_groups) * chunks + warps - 1) / warps, kSortThreads, 0,
-                            s, p);
+                            ((groups + p.tokens) * chunks + warps - 1) / warps, kSortThreads, 0, s,
+                            p);
   }
-  const int64_t chunks = (p.cols + 32 * VEC - 1) / (32 * VEC);
-  return launch_dependent(&nvfp4_combine_tokens_kernel<T, VEC>,
-                          (p.tokens * chunks + warps - 1) / warps, kSortThreads, 0, s, p);
+  // A whole row per block where the tokens alone fill the GPU, parts of it where they do not.
+  const int span = kTokenThreads * VEC * kTokenPieces;
+  const int64_t chunks = (p.cols + span - 1) / span;
+  const int64_t parts = std::min<int64_t>(
+      chunks, std::max<int64_t>(1, static_cast<int64_t>(num_sms) * 8 / p.tokens));
+  return launch_dependent(&nvfp4_combine_tokens_kernel<T, VEC>, p.tokens * parts, kTokenThreads, 0, s,
+                          p, static_cast<int>(parts));
 }
 
 int run(SortOp op, int dtype, const TokenSortParams& p, void* stream) {
@@ -60,11 +67,11 @@ int run(SortOp op, int dtype, const TokenSortParams& p, void* stream) {
                    vector_rows(p.y, p.ldy, es) && vector_rows(p.out, p.ldo, es);
   cudaError_t e;
   if (dtype == NVFP4_DTYPE_FP32)
-    e = vec ? launch<float, 4>(op, p, s) : launch<float, 1>(op, p, s);
+    e = vec ? launch<float, 4>(op, p, ds->num_sms, s) : launch<float, 1>(op, p, ds->num_sms, s);
   else if (dtype == NVFP4_DTYPE_FP16)
-    e = vec ? launch<__half, 8>(op, p, s) : launch<__half, 1>(op, p, s);
+    e = vec ? launch<__half, 8>(op, p, ds->num_sms, s) : launch<__half, 1>(op, p, ds->num_sms, s);
   else
-    e = vec ? launch<__nv_bfloat16, 8>(op, p, s) : launch<__nv_bfloat16, 1>(op, p, s);
+    e = vec ? launch<__nv_bfloat16, 8>(op, p, ds->num_sms, s) : launch<__nv_bfloat16, 1>(op, p, ds->num_sms, s);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "token sort launch");
 }
 

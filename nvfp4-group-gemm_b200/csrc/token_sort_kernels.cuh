@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "sm100_ptx.cuh"
 
@@ -36,36 +37,6 @@ struct TokenSortParams {
   int32_t tokens, topk, cols, rows;
 };
 
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Piece {
-  T v[VEC];
-};
-
-template <typename T, int VEC>
-__device__ __forceinline__ Piece<T, VEC> load_piece(const T* p) {
-  Piece<T, VEC> r;
-  if constexpr (VEC == 1) {
-    r.v[0] = *p;
-  } else {
-    *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
-  }
-  return r;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
-  if constexpr (VEC == 1) {
-    *p = r.v[0];
-  } else {
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
-  }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ Piece<T, VEC> zero_piece() {
-  Piece<T, VEC> r;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) r.v[i] = T(0.0f);
-  return r;
-}
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -80,27 +51,97 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// VEC consecutive elements: one element, or 16 bytes kept as words until they are used (as
+// arrays of bf16 they took twice the registers).
+template <typename T, int VEC>
+struct Piece {
+  uint4 w;
+  __device__ __forceinline__ float get(int i) const {
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(words[i]);
+    } else {
+      const uint32_t v = words[i / 2];
+      if constexpr (std::is_same<T, __half>::value)
+        return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? v >> 16 : v & 0xffffu)));
+      else
+        return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[VEC]) {
+    uint32_t words[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        words[k] = __float_as_uint(f[k]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+        words[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+        words[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    w = make_uint4(words[0], words[1], words[2], words[3]);
+  }
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+  __device__ __forceinline__ void clear() { w = make_uint4(0u, 0u, 0u, 0u); }
+};
+template <typename T>
+struct Piece<T, 1> {
+  T v;
+  __device__ __forceinline__ float get(int) const { return to_f32(v); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { v = from_f32<T>(f[0]); }
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(p); }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ void clear() { v = from_f32<T>(0.0f); }
+};
+
 constexpr int kSortThreads = 256;
 constexpr int kSortPieces = 4;  // pieces a lane moves per task, all loaded before the first store
 
-// Zero columns [c0, c0 + span) of the padding rows among rows [32 g, 32 g + 32). Warp-wide.
+// The row and weight of up to eight slots of a token, from slot j0 on; row -1: dropped or past
+// the last slot.
+struct Slots {
+  int32_t row[8];
+  float w[8];
+};
+__device__ __forceinline__ Slots load_slots(const TokenSortParams& p, int64_t t, int j0) {
+  Slots s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool in = t < p.tokens && j0 + j < p.topk;
+    s.row[j] = in ? __ldg(p.dest + t * p.topk + j0 + j) : -1;
+    s.w[j] = in && p.weights != nullptr ? __ldg(p.weights + t * p.topk + j0 + j) : 1.0f;
+    if (s.row[j] >= p.rows) s.row[j] = -1;
+  }
+  return s;
+}
+
+constexpr int kPadRows = 16;  // rows whose padding one task clears (32: 7.4 us for 300 x 4 pairs)
+
+// Zero columns [c0, c0 + span) of the padding rows among rows [kPadRows g, kPadRows (g + 1)).
+// Warp-wide.
 template <typename T, int VEC>
 __device__ __forceinline__ void zero_padding(const TokenSortParams& p, int64_t g, int c0, int span,
                                              int lane) {
-  const int64_t r = g * 32 + lane;
-  uint32_t pad = __ballot_sync(0xffffffffu, r < p.rows && __ldg(p.src_rows + r) < 0);
+  const int64_t r = g * kPadRows + lane;
+  uint32_t pad = __ballot_sync(0xffffffffu,
+                               lane < kPadRows && r < p.rows && __ldg(p.src_rows + r) < 0);
   const int c1 = min(p.cols, c0 + span);
-  const Piece<T, VEC> z = zero_piece<T, VEC>();
+  Piece<T, VEC> z;
+  z.clear();
   while (pad != 0u) {
     const int i = __ffs(pad) - 1;
     pad &= pad - 1;
-    T* row = static_cast<T*>(p.out) + (g * 32 + i) * p.ldo;
-    for (int c = c0 + lane * VEC; c < c1; c += 32 * VEC) store_piece<T, VEC>(row + c, z);
+    T* row = static_cast<T*>(p.out) + (g * kPadRows + i) * p.ldo;
+    for (int c = c0 + lane * VEC; c < c1; c += 32 * VEC) z.store(row + c);
   }
 }
 
-// One warp per (token, 32 * VEC * kSortPieces columns), then one per (32 rows, as many columns)
-// for the padding.
+// One warp per (kPadRows rows, 32 * VEC * kSortPieces columns) for the padding, then one per
+// (token, as many columns).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSortThreads)
     nvfp4_dispatch_tokens_kernel(const __grid_constant__ TokenSortParams p) {
@@ -109,129 +150,170 @@ __global__ void __launch_bounds__(kSortThreads)
   constexpr int kSpan = 32 * VEC * kSortPieces;
   const int lane = threadIdx.x & 31;
   const int chunks = (p.cols + kSpan - 1) / kSpan;
+  const int64_t groups = (static_cast<int64_t>(p.rows) + kPadRows - 1) / kPadRows;
   const int64_t task = (static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x) >> 5;
-  const int64_t t = task / chunks;
+  const int64_t t = task / chunks - groups;
   const int c0 = static_cast<int>(task % chunks) * kSpan;
-  if (t >= p.tokens) {
-    const int64_t g = t - p.tokens;
-    if (g * 32 < p.rows) zero_padding<T, VEC>(p, g, c0, kSpan, lane);
+  if (t < 0) {
+    zero_padding<T, VEC>(p, t + groups, c0, kSpan, lane);
     return;
   }
+  if (t >= p.tokens) return;
   const T* row = static_cast<const T*>(p.x) + t * p.ldx;
   Piece<T, VEC> v[kSortPieces];
 #pragma unroll
   for (int u = 0; u < kSortPieces; ++u) {
     const int c = c0 + (u * 32 + lane) * VEC;
-    v[u] = c < p.cols ? load_piece<T, VEC>(row + c) : zero_piece<T, VEC>();
+    v[u].clear();
+    if (c < p.cols) v[u].load(row + c);
   }
-  for (int j = 0; j < p.topk; ++j) {
-    const int64_t d = __ldg(p.dest + t * p.topk + j);
-    if (d < 0 || d >= p.rows) continue;
-    T* out = static_cast<T*>(p.out) + d * p.ldo;
+  for (int j0 = 0; j0 < p.topk; j0 += 8) {
+    const Slots s = load_slots(p, t, j0);
 #pragma unroll
-    for (int u = 0; u < kSortPieces; ++u) {
-      const int c = c0 + (u * 32 + lane) * VEC;
-      if (c < p.cols) store_piece<T, VEC>(out + c, v[u]);
+    for (int j = 0; j < 8; ++j) {
+      if (s.row[j] < 0) continue;
+      T* out = static_cast<T*>(p.out) + s.row[j] * p.ldo;
+#pragma unroll
+      for (int u = 0; u < kSortPieces; ++u) {
+        const int c = c0 + (u * 32 + lane) * VEC;
+        if (c < p.cols) v[u].store(out + c);
+      }
     }
   }
 }
 
-// One warp per (token, 32 * VEC columns); up to eight slots' rows are loaded before the first
-// is added.
+// Combine and its gradients: small blocks, one token each. A lane holds kTokenPieces pieces of
+// every one of eight slots' rows at once, so a warp has 8 KB in flight, and short-lived blocks
+// keep the SMs evenly loaded: at 8192 tokens x 8 slots x 4096 bf16 columns the gradients took
+// 180 us like this (0.99 of the measured copy rate), 225 with as many persistent blocks as fit,
+// 201 with blocks of 128 and one piece per lane, 235 with blocks of 256.
+constexpr int kTokenThreads = 64;
+constexpr int kTokenPieces = 2;
+
+// Block b works on token b / parts, on every parts-th chunk of its columns.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kSortThreads)
-    nvfp4_combine_tokens_kernel(const __grid_constant__ TokenSortParams p) {
+__global__ void __launch_bounds__(kTokenThreads)
+    nvfp4_combine_tokens_kernel(const __grid_constant__ TokenSortParams p, int parts) {
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  constexpr int kSpan = 32 * VEC;
+  constexpr int P = kTokenPieces;
+  constexpr int kSpan = kTokenThreads * VEC * P;  // columns of a chunk
   const int lane = threadIdx.x & 31;
-  const int chunks = (p.cols + kSpan - 1) / kSpan;
-  const int64_t task = (static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x) >> 5;
-  const int64_t t = task / chunks;
-  const int c = static_cast<int>(task % chunks) * kSpan + lane * VEC;
-  if (t >= p.tokens || c >= p.cols) return;
+  const int warp = threadIdx.x >> 5;
+  const int64_t t = blockIdx.x / parts;
   const T* y = static_cast<const T*>(p.x);
-  float acc[VEC];
+  const Slots first = load_slots(p, t, 0);
+  for (int c0 = static_cast<int>(blockIdx.x % parts) * kSpan + (warp * 32 * P + lane) * VEC;
+       c0 < p.cols; c0 += parts * kSpan) {
+    float acc[P][VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-  for (int j0 = 0; j0 < p.topk; j0 += 8) {
-    int64_t d[8];
-    Piece<T, VEC> v[8];
-    float w[8];
+    for (int u = 0; u < P; ++u)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d[j] = j0 + j < p.topk ? __ldg(p.dest + t * p.topk + j0 + j) : -1;
-      if (d[j] >= p.rows) d[j] = -1;
-      w[j] = d[j] >= 0 && p.weights != nullptr ? __ldg(p.weights + t * p.topk + j0 + j) : 1.0f;
+      for (int i = 0; i < VEC; ++i) acc[u][i] = 0.0f;
+    for (int j0 = 0; j0 < p.topk; j0 += 8) {
+      const Slots s = j0 == 0 ? first : load_slots(p, t, j0);
+      Piece<T, VEC> v[8][P];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+          const int c = c0 + u * 32 * VEC;
+          if (s.row[j] >= 0 && c < p.cols) v[j][u].load(y + s.row[j] * p.ldx + c);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (s.row[j] < 0) continue;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            acc[u][i] = __fadd_rn(acc[u][i], __fmul_rn(s.w[j], v[j][u].get(i)));
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (d[j] >= 0) v[j] = load_piece<T, VEC>(y + d[j] * p.ldx + c);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (d[j] < 0) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        acc[i] = __fadd_rn(acc[i], __fmul_rn(w[j], to_f32(v[j].v[i])));
+    for (int u = 0; u < P; ++u) {
+      const int c = c0 + u * 32 * VEC;
+      if (c < p.cols) {
+        Piece<T, VEC> o;
+        o.set(acc[u]);
+        o.store(static_cast<T*>(p.out) + t * p.ldo + c);
+      }
     }
   }
-  Piece<T, VEC> o;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(acc[i]);
-  store_piece<T, VEC>(static_cast<T*>(p.out) + t * p.ldo + c, o);
 }
 
-// One block per token; blocks behind the tokens zero the padding of 32 rows each.
+// The first blocks clear the padding, kPadRows rows each; the others take one token each.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kSortThreads)
+__global__ void __launch_bounds__(kTokenThreads)
     nvfp4_combine_tokens_backward_kernel(const __grid_constant__ TokenSortParams p) {
-  constexpr int kWarps = kSortThreads / 32;
+  constexpr int kWarps = kTokenThreads / 32;
+  constexpr int P = kTokenPieces;
+  constexpr int kSpan = kTokenThreads * VEC * P;
   __shared__ float part[kWarps][8];
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  if (t >= p.tokens) {
+  const T* y = static_cast<const T*>(p.y);
+  T* dy = static_cast<T*>(p.out);
+  const int64_t groups =
+      dy != nullptr ? (static_cast<int64_t>(p.rows) + kPadRows - 1) / kPadRows : 0;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) - groups;
+  if (t < 0) {
     const int span = ((p.cols + kWarps - 1) / kWarps + 32 * VEC - 1) / (32 * VEC) * (32 * VEC);
-    if (warp * span < p.cols) zero_padding<T, VEC>(p, t - p.tokens, warp * span, span, lane);
+    zero_padding<T, VEC>(p, t + groups, warp * span, span, lane);
     return;
   }
   const T* g = static_cast<const T*>(p.x) + t * p.ldx;
-  const T* y = static_cast<const T*>(p.y);
-  T* dy = static_cast<T*>(p.out);
   for (int j0 = 0; j0 < p.topk; j0 += 8) {
-    int64_t d[8];
-    float w[8], acc[8];
+    const Slots s = load_slots(p, t, j0);
+    float acc[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d[j] = j0 + j < p.topk ? __ldg(p.dest + t * p.topk + j0 + j) : -1;
-      if (d[j] >= p.rows) d[j] = -1;
-      w[j] = d[j] >= 0 && p.weights != nullptr ? __ldg(p.weights + t * p.topk + j0 + j) : 1.0f;
-      acc[j] = 0.0f;
-    }
-    for (int c = threadIdx.x * VEC; c < p.cols; c += kSortThreads * VEC) {
-      const Piece<T, VEC> gv = load_piece<T, VEC>(g + c);
+    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+    for (int c0 = (warp * 32 * P + lane) * VEC; c0 < p.cols; c0 += kSpan) {
+      Piece<T, VEC> gv[P];
+      Piece<T, VEC> v[8][P];
+#pragma unroll
+      for (int u = 0; u < P; ++u) {
+        const int c = c0 + u * 32 * VEC;
+        gv[u].clear();
+        if (c < p.cols) gv[u].load(g + c);
+      }
       if (p.grad_w != nullptr) {
-        Piece<T, VEC> v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (d[j] >= 0) v[j] = load_piece<T, VEC>(y + d[j] * p.ldy + c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (d[j] < 0) continue;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc[j] += to_f32(gv.v[i]) * to_f32(v[j].v[i]);
-        }
+          for (int u = 0; u < P; ++u) {
+            const int c = c0 + u * 32 * VEC;
+            if (s.row[j] >= 0 && c < p.cols) v[j][u].load(y + s.row[j] * p.ldy + c);
+          }
       }
       if (dy != nullptr) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (d[j] < 0) continue;
-          Piece<T, VEC> o;
+          if (s.row[j] < 0) continue;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(__fmul_rn(w[j], to_f32(gv.v[i])));
-          store_piece<T, VEC>(dy + d[j] * p.ldo + c, o);
+          for (int u = 0; u < P; ++u) {
+            const int c = c0 + u * 32 * VEC;
+            float f[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = __fmul_rn(s.w[j], gv[u].get(i));
+            Piece<T, VEC> o;
+            o.set(f);
+            if (c < p.cols) o.store(dy + s.row[j] * p.ldo + c);
+          }
+        }
+      }
+      if (p.grad_w != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (s.row[j] < 0) continue;
+#pragma unroll
+          for (int u = 0; u < P; ++u) {
+            if (c0 + u * 32 * VEC >= p.cols) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[j] += gv[u].get(i) * v[j][u].get(i);
+          }
         }
       }
     }
@@ -239,7 +321,7 @@ __global__ void __launch_bounds__(kSortThreads)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], s);
+        for (int d = 16; d > 0; d >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], d);
         if (lane == 0) part[warp][j] = acc[j];
       }
       __syncthreads();
