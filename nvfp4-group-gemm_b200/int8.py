@@ -137,12 +137,12 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor | None = None,
     return codes, scales
 
 
-def _out_for(out, out_dtype, rows: int, n: int, device) -> torch.Tensor:
+def _out_for(out, out_dtype, rows: int, n: int, like) -> torch.Tensor:
     if out is None:
         dtype = torch.bfloat16 if out_dtype is None else out_dtype
         if dtype not in _OUT_DTYPES:
             raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {dtype}")
-        return torch.empty((rows, n), dtype=dtype, device=device)
+        return like.new_empty((rows, n), dtype=dtype)
     return out
 
 
@@ -160,18 +160,14 @@ def _check_out(out, out_dtype, rows: int, n: int) -> None:
 
 def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, n, k, experts, offsets,
              counts, expected_rows, stream) -> None:
-    p = _native.Int8Product()
-    p.a, p.lda, p.a_scale = a.data_ptr(), lda, a_scale.data_ptr()
-    p.b, p.ldb, p.b_scale = b.data_ptr(), ldb, b_scale.data_ptr()
-    if b2 is not None:
-        p.b2, p.b2_scale = b2.data_ptr(), b2_scale.data_ptr()
-    if bias is not None:
-        p.bias = bias.data_ptr()
-    if offsets is not None:
-        p.seg_offsets, p.seg_counts = offsets.data_ptr(), counts.data_ptr()
-    p.out, p.ldo, p.out_dtype = out.data_ptr(), _row_stride(out), _OUT_DTYPES[out.dtype]
-    p.rows, p.n, p.k, p.num_experts = int(a.shape[0]), n, k, experts
-    p.expected_rows = expected_rows
+    rows = a.shape[0]
+    p = _native.Int8Product(  # positional: the fields in their order
+        a.data_ptr(), b.data_ptr(), b2.data_ptr() if b2 is not None else None, a_scale.data_ptr(),
+        b_scale.data_ptr(), b2_scale.data_ptr() if b2 is not None else None,
+        bias.data_ptr() if bias is not None else None, out.data_ptr(),
+        offsets.data_ptr() if offsets is not None else None,
+        counts.data_ptr() if counts is not None else None, rows, lda, ldb, _row_stride(out),
+        expected_rows, n, k, experts, _OUT_DTYPES[out.dtype])
     lib = _native.load_library()
     _native.check(lib.nvfp4_int8_gemm(ctypes.byref(p), stream), lib)
 
@@ -188,7 +184,8 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     any row stride and alignment.
     """
     lda, ldb = _codes_stride(a, "a"), _codes_stride(b, "b")
-    m, n, k = int(a.shape[0]), int(b.shape[0]), int(a.shape[1])
+    m, k = a.shape
+    n = b.shape[0]
     if b.shape[1] != k or n < 1:
         raise ValueError(f"b must be [N >= 1, {k}], got {list(b.shape)}")
     if k > _native.INT8_MAX_K:
@@ -200,7 +197,7 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     _check_out(out, out_dtype, m, n)
     s, where = _launch_on((a, a_scale, b, b_scale, bias, out), stream)
     with where:
-        out = _out_for(out, out_dtype, m, n, a.device)
+        out = _out_for(out, out_dtype, m, n, a)
         _product(a, lda, a_scale, b, ldb, b_scale, None, None, bias, out, n, k, 1, None, None, 0, s)
     return out
 
@@ -259,7 +256,7 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     _check_out(out, out_dtype, rows, n)
     s, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out), stream)
     with where:
-        out = _out_for(out, out_dtype, rows, n, a.device)
+        out = _out_for(out, out_dtype, rows, n, a)
         _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out, n, k, experts,
                  seg_offsets, seg_counts, int(expected_rows), s)
     return out

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .int8 import _OUT_DTYPES, _launch_on, _row_stride, _unit_inner
+from .int8 import _OUT_DTYPES, _launch_on
 
 
 def _check_routing(routing) -> tuple:
@@ -39,11 +39,16 @@ def _check_rows(t: torch.Tensor, rows: int, name: str, cols: int | None = None) 
         raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
 
 
-def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy where its rows overlap (expanded tensors) or are not contiguous."""
-    if not _unit_inner(t) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
+def _rows_of(t: torch.Tensor) -> tuple:
+    """``(tensor, row stride)``: ``t``, or a copy where its rows overlap (expanded tensors) or are
+    not contiguous."""
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if inner == 1 and ld >= cols:
+        return t, ld
+    if rows <= 1 and (inner == 1 or cols == 1):
+        return t, cols
+    return t.contiguous(), cols
 
 
 def _fp32(weights):
@@ -56,24 +61,59 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _dispatch(x, routing, stream):
-    tokens, topk, rows, dest, src = _check_routing(routing)
-    _check_rows(x, tokens, "x")
-    s, where = _launch_on((x, dest, src), stream)
-    with where:
-        x = _rows_of(x)
-        cols = int(x.shape[1])
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        lib = _native.load_library()
-        _native.check(lib.nvfp4_moe_dispatch_tokens(
-            x.data_ptr(), _row_stride(x), _OUT_DTYPES[x.dtype], dest.data_ptr(), src.data_ptr(),
-            tokens, topk, cols, rows, y.data_ptr(), cols, s), lib)
+# The launches, on checked arguments; `sizes` is (tokens, topk, rows) of the routing.
+def _launch_dispatch(x, dest, src, sizes, raw_stream):
+    tokens, topk, rows = sizes
+    x, ld = _rows_of(x)
+    cols = x.shape[1]
+    y = x.new_empty((rows, cols))
+    lib = _native.load_library()
+    _native.check(lib.nvfp4_moe_dispatch_tokens(
+        x.data_ptr(), ld, _OUT_DTYPES[x.dtype], dest.data_ptr(), src.data_ptr(), tokens, topk, cols,
+        rows, y.data_ptr(), cols, raw_stream), lib)
     return y
+
+
+def _launch_combine(y, dest, weights, sizes, raw_stream):
+    tokens, topk, rows = sizes
+    y, ld = _rows_of(y)
+    w = _fp32(weights)
+    cols = y.shape[1]
+    out = y.new_empty((tokens, cols))
+    lib = _native.load_library()
+    _native.check(lib.nvfp4_moe_combine_tokens(
+        y.data_ptr(), ld, _OUT_DTYPES[y.dtype], dest.data_ptr(), _ptr(w), tokens, topk, cols, rows,
+        out.data_ptr(), cols, raw_stream), lib)
+    return out
+
+
+def _launch_combine_backward(g, y, dest, src, weights, sizes, want_y, raw_stream):
+    """Gradients of the rows (or None) and, where ``y`` is given, of the weights."""
+    tokens, topk, rows = sizes
+    g, ldg = _rows_of(g)
+    y, ldy = _rows_of(y) if y is not None else (None, 0)
+    w = _fp32(weights)
+    cols = g.shape[1]
+    gy = g.new_empty((rows, cols)) if want_y else None
+    gw = g.new_empty((tokens, topk), dtype=torch.float32) if y is not None else None
+    lib = _native.load_library()
+    _native.check(lib.nvfp4_moe_combine_tokens_backward(
+        g.data_ptr(), ldg, _ptr(y), ldy, _OUT_DTYPES[g.dtype], dest.data_ptr(), src.data_ptr(),
+        _ptr(w), tokens, topk, cols, rows, _ptr(gy), cols, _ptr(gw), raw_stream), lib)
+    return gy, gw
 
 
 def _check_weights(weights, tokens, topk):
     if tuple(weights.shape) != (tokens, topk) or not weights.is_floating_point():
         raise ValueError(f"weights must be a floating-point tensor [{tokens}, {topk}]")
+
+
+def _dispatch(x, routing, stream):
+    tokens, topk, rows, dest, src = _check_routing(routing)
+    _check_rows(x, tokens, "x")
+    s, where = _launch_on((x, dest, src), stream)
+    with where:
+        return _launch_dispatch(x, dest, src, (tokens, topk, rows), s)
 
 
 def _combine(y, routing, weights, stream):
@@ -83,15 +123,7 @@ def _combine(y, routing, weights, stream):
         _check_weights(weights, tokens, topk)
     s, where = _launch_on((y, dest, weights), stream)
     with where:
-        y = _rows_of(y)
-        w = _fp32(weights)
-        cols = int(y.shape[1])
-        out = torch.empty((tokens, cols), dtype=y.dtype, device=y.device)
-        lib = _native.load_library()
-        _native.check(lib.nvfp4_moe_combine_tokens(
-            y.data_ptr(), _row_stride(y), _OUT_DTYPES[y.dtype], dest.data_ptr(), _ptr(w), tokens,
-            topk, cols, rows, out.data_ptr(), cols, s), lib)
-    return out
+        return _launch_combine(y, dest, weights, (tokens, topk, rows), s)
 
 
 def dispatch_tokens_backward(grad_y: torch.Tensor, routing,
@@ -112,78 +144,72 @@ def combine_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor | None, rout
     """
     tokens, topk, rows, dest, src = _check_routing(routing)
     _check_rows(grad_out, tokens, "grad_out")
-    cols = int(grad_out.shape[1])
     if want_weights:
         if y is None:
             raise ValueError("the gradient of the weights needs y")
-        _check_rows(y, rows, "y", cols)
+        _check_rows(y, rows, "y", int(grad_out.shape[1]))
         if y.dtype != grad_out.dtype:
             raise ValueError(f"y is {y.dtype}, grad_out is {grad_out.dtype}")
     if weights is not None:
         _check_weights(weights, tokens, topk)
-    used_y = y if want_weights else None
-    s, where = _launch_on((grad_out, dest, src, weights, used_y), stream)
+    y = y if want_weights else None
+    s, where = _launch_on((grad_out, dest, src, weights, y), stream)
     with where:
-        g = _rows_of(grad_out)
-        used_y = _rows_of(used_y) if want_weights else None
-        w = _fp32(weights)
-        dev = g.device
-        gy = torch.empty((rows, cols), dtype=g.dtype, device=dev) if want_y else None
-        gw = torch.empty((tokens, topk), dtype=torch.float32, device=dev) if want_weights else None
-        lib = _native.load_library()
-        _native.check(lib.nvfp4_moe_combine_tokens_backward(
-            g.data_ptr(), _row_stride(g), _ptr(used_y), _row_stride(used_y) if want_weights else 0,
-            _OUT_DTYPES[g.dtype], dest.data_ptr(), src.data_ptr(), _ptr(w), tokens, topk, cols, rows,
-            _ptr(gy), cols, _ptr(gw), s), lib)
-    return gy, gw
+        return _launch_combine_backward(grad_out, y, dest, src, weights, (tokens, topk, rows), want_y,
+                                        s)
 
 
 class _Kept:
-    """The parts of a Routing a gradient needs (its tensors come back from the saved ones)."""
+    """A Routing's parts that the gradients need."""
 
-    def __init__(self, routing, dest, src_rows):
-        self.tokens, self.topk, self.rows = int(routing.tokens), int(routing.topk), int(routing.rows)
+    def __init__(self, sizes, dest, src_rows):
+        self.tokens, self.topk, self.rows = sizes
         self.dest, self.src_rows = dest, src_rows
 
 
+# The backward passes run on the device and stream of their forward pass (autograd sees to it),
+# with gradients of the outputs' shape, type and device.
 class _DispatchTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, routing):
-        ctx.routing = _Kept(routing, None, None)
-        ctx.save_for_backward(routing.dest, routing.src_rows)
+        dest, src = routing.dest, routing.src_rows
+        ctx.sizes = (int(routing.tokens), int(routing.topk), int(routing.rows))
+        ctx.save_for_backward(dest, src)
         return _dispatch(x, routing, None)
 
     @staticmethod
     def backward(ctx, grad_y):
-        ctx.routing.dest, ctx.routing.src_rows = ctx.saved_tensors
+        dest, src = ctx.saved_tensors
         if torch.is_grad_enabled():  # the gradient of the gradient: the same two operators again
-            return combine_tokens(grad_y, ctx.routing), None
-        return _combine(grad_y, ctx.routing, None, None), None
+            return combine_tokens(grad_y, _Kept(ctx.sizes, dest, src)), None
+        raw = torch._C._cuda_getCurrentRawStream(grad_y.get_device())
+        return _launch_combine(grad_y, dest, None, ctx.sizes, raw), None
 
 
 def _combine_gradients(ctx, grad_out):
     dest, src, weights, y = ctx.saved_tensors
-    ctx.routing.dest, ctx.routing.src_rows = dest, src
-    gy, gw = combine_tokens_backward(grad_out, y, ctx.routing, weights,
-                                     want_y=ctx.needs_input_grad[0], want_weights=y is not None)
-    return gy, gw.to(weights.dtype) if gw is not None else None, None
+    raw = torch._C._cuda_getCurrentRawStream(grad_out.get_device())
+    gy, gw = _launch_combine_backward(grad_out, y, dest, src, weights, ctx.sizes,
+                                      ctx.needs_input_grad[0], raw)
+    if gw is not None and gw.dtype != weights.dtype:
+        gw = gw.to(weights.dtype)
+    return gy, gw, None
 
 
 class _CombineTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, routing):
         want_w = weights is not None and ctx.needs_input_grad[1]
-        ctx.routing = _Kept(routing, None, None)
+        ctx.sizes = (int(routing.tokens), int(routing.topk), int(routing.rows))
         ctx.save_for_backward(routing.dest, routing.src_rows, weights, y if want_w else None)
         return _combine(y, routing, weights, None)
 
     @staticmethod
     def backward(ctx, grad_out):
         if torch.is_grad_enabled():
-            if ctx.saved_tensors[2] is None:
-                dest, src = ctx.saved_tensors[:2]
-                ctx.routing.dest, ctx.routing.src_rows = dest, src
-                return dispatch_tokens(grad_out, ctx.routing), None, None
+            dest, src, weights, _ = ctx.saved_tensors
+            if weights is None:
+                return dispatch_tokens(grad_out, _Kept(ctx.sizes, dest, src)), None, None
             return once_differentiable(_combine_gradients)(ctx, grad_out)
         return _combine_gradients(ctx, grad_out)
 
