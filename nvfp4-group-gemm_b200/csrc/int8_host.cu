@@ -192,6 +192,20 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
   return launch_int8<128, GATED>(g, p, num_sms, s);
 }
 
+template <typename T>
+cudaError_t launch_quantize_int8(const Int8QuantParams& p, cudaStream_t s) {
+  auto go = [&](auto kernel, int group) {
+    const int64_t per_block = kInt8QuantThreads / group;
+    return launch_dependent(kernel, (p.rows + per_block - 1) / per_block, kInt8QuantThreads, 0, s, p);
+  };
+  const int per_thread = kInt8Chunk * kInt8Chunks;
+  const int need = (p.cols + per_thread - 1) / per_thread;  // threads that hold a row
+  if (need <= 32) return go(&nvfp4_quantize_int8_kernel<T, 32>, 32);
+  if (need <= 64) return go(&nvfp4_quantize_int8_kernel<T, 64>, 64);
+  if (need <= 128) return go(&nvfp4_quantize_int8_kernel<T, 128>, 128);
+  return go(&nvfp4_quantize_int8_kernel<T, 256>, 256);
+}
+
 int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
                        const int32_t* row_mask, const int32_t* dest, int topk, int64_t out_rows,
                        void* codes, int64_t codes_ld, float* scales, void* stream) {
@@ -216,7 +230,8 @@ int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dt
   p.ld = ld;
   p.rows = static_cast<int32_t>(rows);
   p.cols = cols;
-  p.vec = aligned16(x) && ld % 8 == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+  p.align = at % 16 == 0 && ld % 8 == 0 ? 16 : at % 4 == 0 && ld % 2 == 0 ? 4 : 2;
   p.row_mask = row_mask;
   p.dest = dest;
   p.topk = topk;
@@ -225,23 +240,9 @@ int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dt
   p.codes_ld = codes_ld;
   p.scales = scales;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int per_thread = kInt8Chunk * kInt8ChunksPerThread;
-  const int need = (cols + per_thread - 1) / per_thread;  // threads that hold a row
-  auto go = [&](auto kernel, int group) {
-    const int64_t per_block = kInt8QuantThreads / group;
-    return launch_dependent(kernel, (rows + per_block - 1) / per_block, kInt8QuantThreads, 0, s, p);
-  };
-  cudaError_t e;
-  if (dtype == NVFP4_DTYPE_BF16)
-    e = need <= 32   ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 32>, 32)
-        : need <= 64 ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 64>, 64)
-        : need <= 128 ? go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 128>, 128)
-                      : go(&nvfp4_quantize_int8_kernel<__nv_bfloat16, 256>, 256);
-  else
-    e = need <= 32   ? go(&nvfp4_quantize_int8_kernel<__half, 32>, 32)
-        : need <= 64 ? go(&nvfp4_quantize_int8_kernel<__half, 64>, 64)
-        : need <= 128 ? go(&nvfp4_quantize_int8_kernel<__half, 128>, 128)
-                      : go(&nvfp4_quantize_int8_kernel<__half, 256>, 256);
+  const cudaError_t e = dtype == NVFP4_DTYPE_BF16
+                            ? launch_quantize_int8<__nv_bfloat16>(p, s)
+                            : launch_quantize_int8<__half>(p, s);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 quantiser launch");
 }
 

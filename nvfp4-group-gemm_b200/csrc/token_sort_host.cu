@@ -15,8 +15,13 @@ int element_size(int dtype) {
   return dtype == NVFP4_DTYPE_FP32 ? 4 : dtype == NVFP4_DTYPE_BF16 || dtype == NVFP4_DTYPE_FP16 ? 2 : 0;
 }
 
-bool vector_rows(const void* p, int64_t ld, int es) {
-  return p == nullptr || (aligned16(p) && ld * es % 16 == 0);
+// Whether rows of `cols` elements move in pieces of `bytes`.
+bool rows_in_pieces(const TokenSortParams& p, int es, int bytes) {
+  auto starts = [&](const void* at, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(at) % bytes == 0 && ld * es % bytes == 0;
+  };
+  return static_cast<int64_t>(p.cols) * es % bytes == 0 && starts(p.x, p.ldx) &&
+         starts(p.y, p.ldy) && starts(p.out, p.ldo);
 }
 
 int check_sizes(int tokens, int topk, int cols, int64_t rows, int dtype, const void* dest) {
@@ -57,21 +62,27 @@ cudaError_t launch(SortOp op, const TokenSortParams& p, int num_sms, cudaStream_
                           p, static_cast<int>(parts));
 }
 
+template <typename T>
+cudaError_t by_piece(SortOp op, int bytes, const TokenSortParams& p, int num_sms, cudaStream_t s) {
+  if (bytes == 16) return launch<T, 16 / sizeof(T)>(op, p, num_sms, s);
+  if (bytes == 8) return launch<T, 8 / sizeof(T)>(op, p, num_sms, s);
+  if constexpr (sizeof(T) == 2)
+    if (bytes == 4) return launch<T, 2>(op, p, num_sms, s);
+  return launch<T, 1>(op, p, num_sms, s);
+}
+
 int run(SortOp op, int dtype, const TokenSortParams& p, void* stream) {
   DeviceState* ds = nullptr;
   const int st = current_device_state(&ds);
   if (st != NVFP4_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int es = element_size(dtype);
-  const bool vec = static_cast<int64_t>(p.cols) * es % 16 == 0 && vector_rows(p.x, p.ldx, es) &&
-                   vector_rows(p.y, p.ldy, es) && vector_rows(p.out, p.ldo, es);
-  cudaError_t e;
-  if (dtype == NVFP4_DTYPE_FP32)
-    e = vec ? launch<float, 4>(op, p, ds->num_sms, s) : launch<float, 1>(op, p, ds->num_sms, s);
-  else if (dtype == NVFP4_DTYPE_FP16)
-    e = vec ? launch<__half, 8>(op, p, ds->num_sms, s) : launch<__half, 1>(op, p, ds->num_sms, s);
-  else
-    e = vec ? launch<__nv_bfloat16, 8>(op, p, ds->num_sms, s) : launch<__nv_bfloat16, 1>(op, p, ds->num_sms, s);
+  const int bytes = rows_in_pieces(p, es, 16) ? 16
+                    : rows_in_pieces(p, es, 8) ? 8
+                    : rows_in_pieces(p, es, 4) ? 4 : 2;
+  const cudaError_t e = dtype == NVFP4_DTYPE_FP32   ? by_piece<float>(op, bytes, p, ds->num_sms, s)
+                        : dtype == NVFP4_DTYPE_FP16 ? by_piece<__half>(op, bytes, p, ds->num_sms, s)
+                                                    : by_piece<__nv_bfloat16>(op, bytes, p, ds->num_sms, s);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "token sort launch");
 }
 

@@ -11,8 +11,9 @@
 // results do not depend on timing. Pairs whose row is outside [0, rows) are dropped pairs.
 // They are bound by memory.
 //
-// Columns move in pieces of 16 bytes (VEC elements) where every row involved starts on a
-// 16-byte boundary, one element at a time otherwise.
+// Columns move in pieces of 16, 8 or 4 bytes (VEC elements), the largest on whose boundaries
+// every row involved starts and that divides the row, or one element at a time (bf16, 8192 x 8
+// pairs of 4095 columns: 0.6 - 0.7 of the copy rate instead of 0.92 and more at 4096).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -51,17 +52,37 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// VEC consecutive elements: one element, or 16 bytes kept as words until they are used (as
+template <int BYTES>
+struct PieceWords;
+template <>
+struct PieceWords<16> { using type = uint4; };
+template <>
+struct PieceWords<8> { using type = uint2; };
+template <>
+struct PieceWords<4> { using type = uint32_t; };
+
+// VEC consecutive elements: one element, or 4 to 16 bytes kept as words until they are used (as
 // arrays of bf16 they took twice the registers).
 template <typename T, int VEC>
 struct Piece {
-  uint4 w;
+  using Words = typename PieceWords<VEC * sizeof(T)>::type;
+  static constexpr int kWords = VEC * sizeof(T) / 4;
+  Words w;
+  __device__ __forceinline__ uint32_t word(int k) const {
+    if constexpr (kWords == 1) return w;
+    else if constexpr (kWords == 2) return k ? w.y : w.x;
+    else return k < 2 ? (k ? w.y : w.x) : (k == 2 ? w.z : w.w);
+  }
+  __device__ __forceinline__ void put(const uint32_t (&k)[kWords]) {
+    if constexpr (kWords == 1) w = k[0];
+    else if constexpr (kWords == 2) w = make_uint2(k[0], k[1]);
+    else w = make_uint4(k[0], k[1], k[2], k[3]);
+  }
   __device__ __forceinline__ float get(int i) const {
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(words[i]);
+      return __uint_as_float(word(i));
     } else {
-      const uint32_t v = words[i / 2];
+      const uint32_t v = word(i / 2);
       if constexpr (std::is_same<T, __half>::value)
         return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? v >> 16 : v & 0xffffu)));
       else
@@ -69,9 +90,9 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void set(const float (&f)[VEC]) {
-    uint32_t words[4];
+    uint32_t words[kWords];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kWords; ++k) {
       if constexpr (sizeof(T) == 4) {
         words[k] = __float_as_uint(f[k]);
       } else if constexpr (std::is_same<T, __half>::value) {
@@ -82,11 +103,16 @@ struct Piece {
         words[k] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    w = make_uint4(words[0], words[1], words[2], words[3]);
+    put(words);
   }
-  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
-  __device__ __forceinline__ void clear() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const Words*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Words*>(p) = w; }
+  __device__ __forceinline__ void clear() {
+    uint32_t zero[kWords];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) zero[k] = 0u;
+    put(zero);
+  }
 };
 template <typename T>
 struct Piece<T, 1> {

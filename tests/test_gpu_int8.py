@@ -80,6 +80,18 @@ def test_quantize_every_ratio_of_ties(pkg, dtype):
     assert np.array_equal(codes.cpu().numpy(), O.quantize_int8(x.double().numpy())[0])
 
 
+@pytest.mark.parametrize("rows,cols", [(2400, 513), (2368, 4096), (2500, 4100), (2371, 8200), (2370, 20000)])
+def test_quantize_many_rows(pkg, rows, cols):
+    """Row counts at which fewer threads share a row."""
+    g = torch.Generator().manual_seed(cols)
+    x = (torch.randn((rows, cols), generator=g) * 3).to(torch.bfloat16)
+    codes, scales = pkg.quantize_int8(x.cuda())
+    xd = x.double()
+    amax = xd.abs().amax(1, keepdim=True)
+    assert torch.equal(codes.cpu(), torch.round(127 * xd / amax).to(torch.int8))
+    assert float(((scales.cpu().double() - amax[:, 0] / 127).abs() / amax[:, 0] * 127).max()) <= U
+
+
 def test_quantize_extreme_rows(pkg):
     x = torch.zeros((8, 40), dtype=torch.bfloat16)
     x[1, 3] = float("inf")

@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: U}
 TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -126}
-CASES = [(1, 1, 1, 8), (1, 1, 1, 1), (37, 2, 8, 515), (64, 4, 16, 512), (5, 9, 12, 96),
+CASES = [(1, 1, 1, 8), (1, 1, 1, 1), (45, 3, 6, 1030), (21, 2, 4, 260), (37, 2, 8, 515), (64, 4, 16, 512), (5, 9, 12, 96),
          (130, 3, 5, 2056), (40, 8, 64, 4096), (6, 17, 20, 33)]
 
 
