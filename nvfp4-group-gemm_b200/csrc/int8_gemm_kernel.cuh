@@ -119,11 +119,14 @@ __device__ __forceinline__ float int8_silu_mul(float g, float u) {
 }
 
 // Segments of the launch in shared memory: first row, rows, and the end of each expert's tile
-// range. Warp-wide; a segment outside the slab is skipped and reported.
+// range. Warp-wide; a segment outside the slab is skipped and reported, and so is one with which
+// the segments hold more rows than the slab (they share some), so that the tiles stay within
+// the host's bound.
 __device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, int tile_rows,
                                                     int n_tiles, int32_t* seg_row,
                                                     int32_t* seg_cnt, int32_t* seg_end, int lane) {
   int32_t carry = 0;
+  int64_t rows_before = 0;
   for (int base = 0; base < p.num_experts; base += 32) {
     const int e = base + lane;
     int32_t off = 0, cnt = 0;
@@ -139,6 +142,17 @@ __device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, int
         }
       }
     }
+    long long sum = cnt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += t;
+    }
+    if (rows_before + sum > p.rows && cnt > 0) {
+      atomicOr(p.error_bits, kDevErrBadSegment);
+      off = cnt = 0;
+    }
+    rows_before += __shfl_sync(0xffffffffu, sum, 31);
     int32_t v = (cnt + tile_rows - 1) / tile_rows * n_tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {

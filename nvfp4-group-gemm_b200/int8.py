@@ -233,7 +233,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     back, so the call can be captured in a CUDA graph. Segments may start anywhere; rows outside
     all of them are left as they were (undefined where ``out`` is allocated here). A segment
     outside the slab is skipped and :func:`check_int8_errors` raises; segments that share rows
-    are not supported. ``expected_rows`` (the host's estimate of all segments' rows, e.g. tokens
+    are not supported (their rows hold either result; segments past the slab's number of rows in
+    all may be skipped and reported). ``expected_rows`` (the host's estimate of all segments' rows, e.g. tokens
     x top-k) picks the tile shape only.
     """
     lda = _codes_stride(a, "a")

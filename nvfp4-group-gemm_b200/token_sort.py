@@ -8,7 +8,12 @@
 bf16, fp16 and fp32, any width and row stride, differentiable in ``x``, the rows and the
 weights (with weights: once). Sums are fp32 in slot order, rounded once: results do not depend on timing.
 The ``*_backward`` functions are the gradients by themselves, for training loops that do not go
-through autograd. The reference has no counterpart.
+through autograd.
+
+Capturing a backward pass in a CUDA graph follows torch's rule: while an eager graph of the same
+leaves is alive, its gradient nodes belong to the stream it was made on, and the capture fails
+with an error. Drop such graphs first, or capture the ``*_backward`` functions, which have no
+such nodes. The reference has no counterpart of this module.
 """
 from __future__ import annotations
 

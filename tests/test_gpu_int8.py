@@ -285,6 +285,35 @@ def test_segment_outside_the_slab_is_skipped_and_reported(pkg):
     assert pkg.check_int8_errors() == 0
 
 
+@pytest.mark.parametrize("expected", [8, 2000])
+def test_segments_that_share_rows_stay_in_bounds(pkg, expected):
+    """Many segments that all claim the whole slab: no row outside them is written, and the
+    excess is reported (few tiles and many)."""
+    rows, n, k, E = 300, 2100, 64, 40
+    a, sa = _codes(rows, k, 1), _scale(rows, 2, 0.01)
+    b, sb = _codes(E * n, k, 3).unflatten(0, (E, n)), _scale((E, n), 4, 0.01)
+    big = torch.full((rows + 20, n), 3.0, dtype=torch.bfloat16, device="cuda")
+    off = torch.zeros(E, dtype=torch.int32, device="cuda")
+    cnt = torch.full((E,), rows, dtype=torch.int32, device="cuda")
+    pkg.int8_gemm_segments(a, sa, b, sb, off, cnt, out=big[10:10 + rows], expected_rows=expected * E)
+    with pytest.raises(pkg.Nvfp4Error, match="segment"):
+        pkg.check_int8_errors()
+    assert torch.all(big[:10] == 3.0) and torch.all(big[10 + rows:] == 3.0)
+
+
+def test_outputs_past_32_bits(pkg):
+    """2.4e9 output elements: the last rows are where they belong."""
+    m, n, k = 600_000, 4000, 16
+    a, sa = _codes(m, k, 1), _scale(m, 2, 0.01)
+    b, sb = _codes(n, k, 3), _scale(n, 4, 0.01)
+    out = pkg.int8_gemm(a, sa, b, sb)
+    for rows in (slice(0, 3), slice(536_869, 536_875), slice(m - 3, m)):
+        _check_product(out[rows], a[rows], sa[rows], b, sb)
+    codes, scales = pkg.quantize_int8(out)
+    want, ws = O.quantize_int8(_np(out[m - 2:]))
+    assert np.array_equal(codes[m - 2:].cpu().numpy(), want)
+
+
 def test_two_streams_and_a_graph(pkg):
     """Calls on two streams at once and two captured graphs, replayed in turn: no shared state."""
     k, n = 512, 384

@@ -108,6 +108,28 @@ def test_gradients_against_differences(pkg):
     assert abs(num - float((gw.double() * dw.double()).sum())) <= tol
 
 
+def test_rows_past_32_bits(pkg):
+    """2.4e9 sorted elements: the last expert's rows and their gradients are where they belong."""
+    tokens, cols = 150_000, 8000
+    ids = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda").repeat(tokens, 1)
+    r = pkg.moe.route(ids, 2)
+    x = torch.arange(tokens, device="cuda", dtype=torch.float32)[:, None].expand(-1, cols)
+    x = (x % 251).to(torch.bfloat16)
+    y = pkg.moe.dispatch_tokens(x, r)
+    for t in (0, 131_072, tokens - 1):
+        for j in range(2):
+            assert torch.equal(y[int(r.dest[2 * t + j])], x[t])
+    w = torch.ones((tokens, 2), device="cuda")
+    gy, gw = pkg.moe.combine_tokens_backward(x, y, r, w)
+    assert torch.equal(gy[int(r.dest[2 * tokens - 1])], x[tokens - 1])
+    t = tokens - 1
+    want = float((x[t].double() ** 2).sum())
+    assert abs(float(gw[t, 1]) - want) <= (cols + 1) * U * want
+    del gy, gw
+    out = pkg.moe.combine_tokens(y, r)
+    assert torch.equal(out[t], (2 * x[t].float()).to(torch.bfloat16))
+
+
 def test_same_expert_twice_and_everything_dropped(pkg):
     ids = torch.tensor([[1, 1], [-1, 7], [0, 1]], dtype=torch.int32, device="cuda")
     r = pkg.moe.route(ids, 2)
