@@ -122,7 +122,7 @@ int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sm
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
-template <int TB, bool GATED>
+template <int TB, int R, int KS, bool GATED>
 int launch_int8_gemv(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sms,
                      cudaStream_t s) {
   Int8GemvParams q = {};
@@ -133,13 +133,27 @@ int launch_int8_gemv(const nvfp4_int8_product* g, const Int8GemmParams& p, int n
   q.lda = g->lda;
   q.ldb = g->ldb;
   q.k = g->k;
-  const int64_t warps =
-      (static_cast<int64_t>(g->n) + kInt8GemvRows - 1) / kInt8GemvRows * g->num_experts;
-  const int64_t blocks = (warps + kInt8GemvThreads / 32 - 1) / (kInt8GemvThreads / 32);
+  const int channels = kInt8GemvThreads / 32 / KS * R;  // of a block
+  const int64_t blocks = (static_cast<int64_t>(g->n) + channels - 1) / channels * g->num_experts;
   const cudaError_t e =
-      launch_dependent(&nvfp4_int8_gemv_kernel<TB, GATED>,
+      launch_dependent(&nvfp4_int8_gemv_kernel<TB, R, KS, GATED>,
                        std::min<int64_t>(blocks, num_sms * 4), kInt8GemvThreads, 0, s, q);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
+}
+
+// Warps of a group (KS): as many as keep the warps within one wave (32 per SM) and leave each
+// two loads of 512 bytes of K. Channels of a group (R): two, four where more tokens' codes have
+// to be loaded for them (four tokens, N 2048, K 2048: 4.0 us against 4.6).
+template <int TB, bool GATED>
+int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p, int64_t active,
+                           int num_sms, cudaStream_t s) {
+  constexpr int R = TB <= 2 || GATED ? 2 : 4;
+  const int64_t groups = (static_cast<int64_t>(g->n) + R - 1) / R * active;
+  auto fits = [&](int ks) { return groups * ks <= num_sms * 32 && g->k >= 1024 * ks; };
+  if (fits(8)) return launch_int8_gemv<TB, R, 8, GATED>(g, p, num_sms, s);
+  if (fits(4)) return launch_int8_gemv<TB, R, 4, GATED>(g, p, num_sms, s);
+  if (fits(2)) return launch_int8_gemv<TB, R, 2, GATED>(g, p, num_sms, s);
+  return launch_int8_gemv<TB, R, 1, GATED>(g, p, num_sms, s);
 }
 
 template <bool GATED>
@@ -162,9 +176,13 @@ int launch_int8_pair(const nvfp4_int8_product* g, const Int8GemmParams& p, int c
 //
 // Few tiles (fewer 128-channel tiles than SMs): a launch takes as long as one CTA's K loop, so
 // the smallest token tile that still runs in one wave is taken. Dense, N 4096, K 7168: 256 rows
-// 13.2 with tiles of 64, 16.5 with 128; 512 rows 16.9 with 128, 21.4 with 64. With one or two
-// rows per expert the weights are streamed by all SMs without tiles (int8_gemv_kernel.cuh):
-// one row 8.6 against 11.4, two rows 11.1 against 11.5; at four rows it loses (17 against 11.5).
+// 13.2 with tiles of 64, 16.5 with 128; 512 rows 16.9 with 128, 21.4 with 64.
+//
+// With at most 8 rows per expert and few tiles the weights are streamed by all SMs without
+// tiles (int8_gemv_kernel.cuh), against these tiles: one row 7.4 and 11.6 us (N 4096, K 7168),
+// 13.7 and 15.6 (N 18432, K 4096); two rows 7.6 and 11.6, 14.1 and 15.4; four rows 10.2 and
+// 11.5, 6.6 and 7.0 (N 7168, K 2048), but 17.5 and 15.5 (N 18432); eight rows 6.4 and 12.1 (N
+// 1024, K 8192), 3.8 and 5.9 (N 2048, K 2048), but 16 and 11.5 (N 4096, K 7168).
 //
 // Many tiles: bound by the weights' bytes while an expert's rows fit one tile, so tiles are
 // chosen to hold them with a quarter to spare (64 experts of 64 +- 8 rows, N 4096, K 1536:
@@ -179,9 +197,17 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
   const int64_t active = std::min<int64_t>(g->num_experts, expected);  // experts with rows
   const int64_t rows = (expected + active - 1) / active;
   const int64_t n_tiles = (g->n + 127) / 128;
-  if (rows <= 2 && active * n_tiles < num_sms)
-    return rows == 1 ? launch_int8_gemv<1, GATED>(g, p, num_sms, s)
-                     : launch_int8_gemv<2, GATED>(g, p, num_sms, s);
+  const int64_t tiles = active * n_tiles;
+  // Experts' counts vary: twice the average, unless each is expected to have one row.
+  const int64_t at_once = g->num_experts > 1 && rows > 1 ? 2 * rows : rows;
+  if (at_once == 1 && tiles < num_sms)
+    return launch_int8_gemv_split<1, GATED>(g, p, active, num_sms, s);
+  if (at_once == 2 && tiles < num_sms)
+    return launch_int8_gemv_split<2, GATED>(g, p, active, num_sms, s);
+  if (at_once <= 4 && (GATED ? 4 : 2) * tiles < num_sms && g->k >= 1024)
+    return launch_int8_gemv_split<4, GATED>(g, p, active, num_sms, s);
+  if (at_once <= 8 && 9 * tiles < num_sms && g->k >= 2048)
+    return launch_int8_gemv_split<8, GATED>(g, p, active, num_sms, s);
   auto one_wave = [&](int tn) { return active * ((rows + tn - 1) / tn) * n_tiles <= num_sms; };
   const bool many = !one_wave(128);
   if (many && rows > 80) return launch_int8_pair<GATED>(g, p, ds.pair_clusters, s);

@@ -160,6 +160,24 @@ def test_product_of_every_kernel(pkg, m, n, k, dtype):
     assert pkg.check_int8_errors() == 0
 
 
+@pytest.mark.parametrize("n,k", [(2000, 8200), (300, 500), (1100, 4096), (500, 2047), (33, 1025)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8])
+def test_product_of_few_rows(pkg, m, n, k):
+    """Few rows and tiles: one to eight tokens at once, K shared by one to eight warps."""
+    a, b = _codes(m, k, 31 + m), _codes(n, k, 32)
+    sa, sb = _scale(m, 33, 0.01), _scale(n, 34, 0.002)
+    _check_product(pkg.int8_gemm(a, sa, b, sb, out_dtype=torch.float16), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("per,k", [(1, 8192), (2, 4100), (3, 2047), (4, 500), (6, 8192), (8, 1030)])
+def test_segments_of_few_rows(pkg, per, k, gated):
+    """The same over experts whose real counts differ from the estimate (one far above it)."""
+    _segments_case(pkg, [40, 0, 7, 30], [per, max(per - 1, 0), 19, 0], 60, 410, k, gated,
+                   torch.bfloat16, 4 * per, seed=per)
+    assert pkg.check_int8_errors() == 0
+
+
 def test_product_sums_are_exact_at_the_largest_k(pkg):
     """Sums next to the edge of int32, and codes of -128."""
     k = pkg._native.INT8_MAX_K
