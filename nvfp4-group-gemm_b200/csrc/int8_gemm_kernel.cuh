@@ -215,6 +215,7 @@ struct Int8Config {
 template <int TN, bool GATED>
 __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
     nvfp4_int8_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                           const __grid_constant__ CUtensorMap map_a32,
                            const __grid_constant__ CUtensorMap map_b,
                            const __grid_constant__ CUtensorMap map_b2,
                            const __grid_constant__ Int8GemmParams p) {
@@ -279,6 +280,11 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
         const Int8Tile t =
             int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
         const int wrow = t.expert * p.n + t.nt * 128;
+        // Tokens come in one box of TN rows, or in boxes of 32 where half the rows are enough.
+        const int boxes = (t.rows + 31) / 32;
+        const bool small = 64 * boxes <= TN;
+        const uint32_t bytes =
+            Cfg::kSets * Cfg::kWBytes + (small ? 32 * boxes * kInt8StageK : Cfg::kXBytes);
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&empty_bar[stage], phase ^ 1u, abort_flag, p.error_bits,
                           kDevErrProducerTimeout)) {
@@ -286,12 +292,17 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
             break;
           }
           uint8_t* sW = smem + stage * Cfg::kStageBytes;
-          ptx::mbar_arrive_expect_tx(&full_bar[stage], Cfg::kStageBytes);
+          ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
           ptx::tma_load_2d(sW, &map_b, &full_bar[stage], kt * kInt8StageK, wrow);
           if (GATED)
             ptx::tma_load_2d(sW + Cfg::kWBytes, &map_b2, &full_bar[stage], kt * kInt8StageK, wrow);
-          ptx::tma_load_2d(sW + Cfg::kSets * Cfg::kWBytes, &map_a, &full_bar[stage],
-                           kt * kInt8StageK, t.row);
+          uint8_t* sX = sW + Cfg::kSets * Cfg::kWBytes;
+          if (small)
+            for (int b = 0; b < boxes; ++b)
+              ptx::tma_load_2d(sX + 32 * b * kInt8StageK, &map_a32, &full_bar[stage],
+                               kt * kInt8StageK, t.row + 32 * b);
+          else
+            ptx::tma_load_2d(sX, &map_a, &full_bar[stage], kt * kInt8StageK, t.row);
           ++issued;
           if (++stage == kStages) {
             stage = 0;

@@ -48,6 +48,7 @@ struct Int8PairConfig {
 template <bool GATED>
 __global__ void __launch_bounds__(kInt8PairThreads, 1)
     nvfp4_int8_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a,
+                                const __grid_constant__ CUtensorMap map_a32,
                                 const __grid_constant__ CUtensorMap map_b,
                                 const __grid_constant__ CUtensorMap map_b2,
                                 const __grid_constant__ Int8GemmParams p) {
@@ -124,6 +125,11 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
         const Int8Tile t = find(tile);
         const int half = mma_n(t) / 2;  // this CTA's tokens
         const int xrow = t.row + rank * half;
+        // In one box of 128 rows, or in boxes of 32 where half the rows are enough.
+        const int boxes = (half + 31) / 32;
+        const bool small = boxes <= 2;
+        const uint32_t bytes =
+            Cfg::kWBytes + (small ? 32 * boxes * kInt8StageK : Cfg::kXBytes);
         const int wrow = t.expert * p.n + t.nt * Cfg::kOutN + rank * Cfg::kWBox;
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&empty_bar[stage], phase ^ 1u, abort_flag, p.error_bits,
@@ -132,14 +138,18 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
             break;
           }
           const uint32_t full = ptx::mapa_shared(ptx::smem_u32(&full_bar[stage]), 0);
-          if (leader) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * Cfg::kStageBytes);
+          if (leader) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2u * bytes);
           uint8_t* sW = smem + stage * Cfg::kStageBytes;
           uint8_t* sX = sW + Cfg::kWBytes;
           const int kx = kt * kInt8StageK;
           ptx::tma_load_2d_pair(sW, &map_b, full, kx, wrow);
           if (GATED)
             ptx::tma_load_2d_pair(sW + Cfg::kWBox * kInt8StageK, &map_b2, full, kx, wrow);
-          ptx::tma_load_2d_pair(sX, &map_a, full, kx, xrow);
+          if (small)
+            for (int b = 0; b < boxes; ++b)
+              ptx::tma_load_2d_pair(sX + 32 * b * kInt8StageK, &map_a32, full, kx, xrow + 32 * b);
+          else
+            ptx::tma_load_2d_pair(sX, &map_a, full, kx, xrow);
           ++issued;
           if (++stage == kStages) {
             stage = 0;

@@ -87,13 +87,14 @@ bool int8_map(CUtensorMap* m, const void* addr, int64_t rows, int k, int64_t ld,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
-// Tensor maps of a product: tokens in boxes of `x_box` rows, weights in boxes of `w_box`.
+// Tensor maps of a product: tokens in boxes of `x_box` and of 32 rows, weights in boxes of `w_box`.
 struct Int8Maps {
-  CUtensorMap a, b, b2;
+  CUtensorMap a, a32, b, b2;
 };
 bool int8_maps(const nvfp4_int8_product* g, int x_box, int w_box, Int8Maps* m) {
   const int64_t wrows = static_cast<int64_t>(g->num_experts) * g->n;
   if (!int8_map(&m->a, g->a, g->rows, g->k, g->lda, x_box) ||
+      !int8_map(&m->a32, g->a, g->rows, g->k, g->lda, 32) ||
       !int8_map(&m->b, g->b, wrows, g->k, g->ldb, w_box))
     return false;
   if (g->b2 == nullptr) {
@@ -118,7 +119,7 @@ int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sm
   if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
       launch_dependent(&nvfp4_int8_gemm_kernel<TN, GATED>, std::min<int64_t>(tiles, num_sms),
-                       Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.b, m.b2, p);
+                       Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
@@ -167,7 +168,7 @@ int launch_int8_pair(const nvfp4_int8_product* g, const Int8GemmParams& p, int c
   if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
       launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED>, std::min<int64_t>(tiles, clusters) * 2,
-                      2, kInt8PairThreads, Cfg::kSmemBytes, s, m.a, m.b, m.b2, p);
+                      2, kInt8PairThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
