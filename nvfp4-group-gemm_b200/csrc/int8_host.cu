@@ -219,18 +219,28 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
   return launch_int8<128, GATED>(g, p, num_sms, s);
 }
 
+template <typename T, int G, int V>
+cudaError_t launch_quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
+  constexpr int kThreads = int8_quant_threads<G>();
+  const int64_t per_block = kThreads / G;
+  return launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V>, (p.rows + per_block - 1) / per_block,
+                          kThreads, 0, s, p);
+}
+
+// The fewest threads that hold a row at four chunks each, or at three where that is as many or
+// fewer (1536 columns: 64 threads, all with columns).
 template <typename T>
 cudaError_t launch_quantize_int8(const Int8QuantParams& p, cudaStream_t s) {
-  auto go = [&](auto kernel, int group) {
-    const int64_t per_block = kInt8QuantThreads / group;
-    return launch_dependent(kernel, (p.rows + per_block - 1) / per_block, kInt8QuantThreads, 0, s, p);
-  };
-  const int per_thread = kInt8Chunk * kInt8Chunks;
-  const int need = (p.cols + per_thread - 1) / per_thread;  // threads that hold a row
-  if (need <= 32) return go(&nvfp4_quantize_int8_kernel<T, 32>, 32);
-  if (need <= 64) return go(&nvfp4_quantize_int8_kernel<T, 64>, 64);
-  if (need <= 128) return go(&nvfp4_quantize_int8_kernel<T, 128>, 128);
-  return go(&nvfp4_quantize_int8_kernel<T, 256>, 256);
+  const int chunks = (p.cols + kInt8Chunk - 1) / kInt8Chunk;
+  if (chunks <= 3 * 32) return launch_quantize_rows<T, 32, 3>(p, s);
+  if (chunks <= 4 * 32) return launch_quantize_rows<T, 32, 4>(p, s);
+  if (chunks <= 3 * 64) return launch_quantize_rows<T, 64, 3>(p, s);
+  if (chunks <= 4 * 64) return launch_quantize_rows<T, 64, 4>(p, s);
+  if (chunks <= 3 * 128) return launch_quantize_rows<T, 128, 3>(p, s);
+  if (chunks <= 4 * 128) return launch_quantize_rows<T, 128, 4>(p, s);
+  if (chunks <= 3 * 256) return launch_quantize_rows<T, 256, 3>(p, s);
+  if (chunks <= 4 * 256) return launch_quantize_rows<T, 256, 4>(p, s);
+  return launch_quantize_rows<T, 512, 4>(p, s);
 }
 
 int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dtype,

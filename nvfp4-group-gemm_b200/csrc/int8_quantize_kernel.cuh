@@ -16,9 +16,8 @@
 // even neighbour there. Rows with maxima far from 1 are scaled by 2^+-64 first, so that 127 / max
 // and 127 x stay in range.
 //
-// Bound by memory: each row is read once and kept in registers between the maximum and the
-// codes (wider rows than a group's registers hold are read again, from L2 by then). With the exact check
-// on every element (13 operations instead of 6) 69,632 rows of 4096 took 244 us.
+// Each row is read once and kept in registers between the maximum and the codes (wider rows than
+// a group's registers hold are read again, from L2 by then).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -30,9 +29,7 @@
 
 namespace nvfp4 {
 
-constexpr int kInt8QuantThreads = 256;
-constexpr int kInt8Chunk = 8;   // columns a thread handles at once: a warp loads 512 bytes in a row
-constexpr int kInt8Chunks = 4;  // chunks a thread keeps in registers
+constexpr int kInt8Chunk = 8;  // columns a thread handles at once: a warp loads 512 bytes in a row
 
 struct Int8QuantParams {
   const uint16_t* x;     // bf16 or fp16 bits
@@ -156,14 +153,18 @@ __device__ __forceinline__ void int8_store_chunk(int8_t* row, int c0, int cols, 
     if (c0 + i < cols) row[c0 + i] = static_cast<int8_t>((i < 4 ? q.x : q.y) >> (8 * (i % 4)));
 }
 
-// G threads per row, kInt8QuantThreads / G rows per block: the smallest group that holds the row
-// in registers, so that many rows are in flight per SM.
-template <typename T, int G>
-__global__ void __launch_bounds__(kInt8QuantThreads, 6)
+// G threads on a row, each with V chunks of it in registers; blocks of one row, or of 128 threads
+// where fewer hold one. Small blocks start and end without waiting for one another: 69,632 rows
+// of 4096 columns took 149 us (0.88 of the measured copy rate) in blocks of 128, 159 in blocks of
+// 256, and 198 with the exact check on every element.
+template <int G>
+__host__ __device__ constexpr int int8_quant_threads() { return G < 128 ? 128 : G; }
+
+template <typename T, int G, int V>
+__global__ void __launch_bounds__(int8_quant_threads<G>(), 1536 / int8_quant_threads<G>())
     nvfp4_quantize_int8_kernel(const __grid_constant__ Int8QuantParams p) {
-  constexpr int kRows = kInt8QuantThreads / G;
-  constexpr int V = kInt8Chunks;
-  __shared__ uint32_t warp_max[kInt8QuantThreads / 32];
+  constexpr int kRows = int8_quant_threads<G>() / G;
+  __shared__ uint32_t warp_max[int8_quant_threads<G>() / 32];
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int group = threadIdx.x / G;
@@ -211,11 +212,11 @@ __global__ void __launch_bounds__(kInt8QuantThreads, 6)
   k.s = s;
   k.amax_s = __fmul_rn(amax, s);
   k.inv = s == 0.0f ? 0.0f : __fdiv_rn(127.0f, k.amax_s);
-  const float scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fc00000u);
+  float scale = 0.0f;  // the group's first thread stores it
+  if (gt == 0) scale = finite ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fc00000u);
   uint2 q[V];
 #pragma unroll
-  for (int u = 0; u < V; ++u)
-    q[u] = int8_codes8<T>(v[u], k);
+  for (int u = 0; u < V; ++u) q[u] = int8_codes8<T>(v[u], k);
   const int copies = p.dest == nullptr ? 1 : p.topk;
   for (int j = 0; j < copies; ++j) {
     const int64_t d = p.dest == nullptr ? r : __ldg(p.dest + r * p.topk + j);

@@ -54,7 +54,7 @@ def _check_product(got, a, sa, b, sb, bias=None):
 # ------------------------------------------------------------------ quantiser
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 17), (5, 16), (9, 1023), (4, 1024), (7, 2050),
-                                       (6, 4096), (3, 8192), (2, 20011), (0, 64), (300, 96)])
+                                       (6, 4096), (3, 8192), (2, 20011), (0, 64), (300, 96), (3, 1300), (5, 2000)])
 def test_quantize_codes_are_those_of_the_exact_quotient(pkg, rows, cols, dtype):
     g = torch.Generator().manual_seed(rows * 7 + cols)
     x = torch.randn((rows, cols), generator=g) * torch.exp(2 * torch.randn((rows, 1), generator=g))
