@@ -104,3 +104,85 @@ def test_training_step_through_the_token_sort(pkg):
     for a, b in zip(got, want):
         rel = float(torch.linalg.norm(a.double() - b) / torch.linalg.norm(b))
         assert rel <= 16 * u * (T * H) ** 0.5, rel
+
+
+def test_block_with_everything_dropped_and_one_expert_twice(pkg):
+    x, gate, up, down, ids, w = _setup(pkg, 20, 2, 4, 64, 32, torch.bfloat16, 2, drop=0.0)
+    W = pkg.moe.quantize_expert_weights_int8(gate, up, down)
+    blk = pkg.moe.Int8MoEBlock(W, 20, 2)
+    first = blk.run(x, ids, w).clone()
+    assert torch.all(blk.run(x, torch.full_like(ids, -1), w) == 0)
+    assert torch.equal(blk.run(x, ids, w), first)  # nothing of the empty run stays
+    twice = ids[:, :1].repeat(1, 2).contiguous()
+    half = torch.full((20, 2), 0.5, device="cuda")
+    both = blk.run(x, twice, half).clone()
+    once = blk.run(x, torch.cat([ids[:, :1], torch.full_like(ids[:, :1], -1)], 1).contiguous(),
+                   torch.ones((20, 2), device="cuda"))
+    assert torch.equal(both, once)  # 0.5 y + 0.5 y is exact
+    assert blk.check_device_errors() == 0
+
+
+def test_block_on_a_stream_of_its_own(pkg):
+    """The caller's stream differs from the current one; weights in another type are converted on it."""
+    x, gate, up, down, ids, w = _setup(pkg, 30, 2, 4, 96, 64, torch.float16, 4)
+    W = pkg.moe.quantize_expert_weights_int8(gate, up, down)
+    blk = pkg.moe.Int8MoEBlock(W, 30, 2, torch.float16)
+    want = blk.run(x, ids, w.to(torch.bfloat16)).clone()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        blk.out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        out = blk.run(x, ids, w.to(torch.bfloat16), stream=side)
+        side.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_operators_on_two_streams_at_once(pkg):
+    """Quantiser, dispatch, products and combine hold no state that two streams could share."""
+    cases = []
+    for seed, (T, H) in enumerate(((500, 512), (33, 1024))):
+        x, gate, up, down, ids, w = _setup(pkg, T, 2, 4, H, 128, torch.bfloat16, seed)
+        W = pkg.moe.quantize_expert_weights_int8(gate, up, down)
+        r = pkg.moe.route(ids, 4)
+        off = torch.tensor(r.offsets[:4], dtype=torch.int32, device="cuda")
+        cnt = torch.tensor(r.counts, dtype=torch.int32, device="cuda")
+        cases.append((x, W, r, off, cnt, w))
+
+    def chain(case, st):
+        x, W, r, off, cnt, w = case
+        a, sa = pkg.moe.dispatch_int8(x, r, stream=st)
+        h = pkg.int8_gemm_segments(a, sa, W.w_gate, W.s_gate, off, cnt, b2=W.w_up, b2_scale=W.s_up,
+                                   stream=st)
+        a2, sa2 = pkg.quantize_int8(h, row_mask=r.src_rows, stream=st)
+        y = pkg.int8_gemm_segments(a2, sa2, W.w_down, W.s_down, off, cnt, stream=st)
+        return pkg.moe.combine_tokens(y, r, w, stream=st)
+
+    want = [chain(c, None) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        got = [chain(c, st) for c, st in zip(cases, streams)]
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_rows_outside_segments_may_hold_anything(pkg):
+    """Padding rows with NaN scales and any codes neither reach a result nor are written."""
+    x, gate, up, down, ids, w = _setup(pkg, 50, 2, 4, 160, 96, torch.bfloat16, 8)
+    W = pkg.moe.quantize_expert_weights_int8(gate, up, down)
+    r = pkg.moe.route(ids, 4)
+    off = torch.tensor(r.offsets[:4], dtype=torch.int32, device="cuda")
+    cnt = torch.tensor(r.counts, dtype=torch.int32, device="cuda")
+    a, sa = pkg.moe.dispatch_int8(x, r)
+    pad = r.src_rows[:r.rows] < 0
+    outs = []
+    for fill, scale in ((0, 0.0), (127, float("nan")), (-128, float("inf"))):
+        a[pad] = fill
+        sa[pad] = scale
+        out = torch.full((r.rows, 96), 7.0, dtype=torch.bfloat16, device="cuda")
+        pkg.int8_gemm_segments(a, sa, W.w_gate, W.s_gate, off, cnt, b2=W.w_up, b2_scale=W.s_up, out=out)
+        assert torch.all(out[pad] == 7.0) and torch.isfinite(out).all()
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
