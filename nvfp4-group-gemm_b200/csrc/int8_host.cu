@@ -223,8 +223,10 @@ template <typename T, int G, int V>
 cudaError_t launch_quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
   constexpr int kThreads = int8_quant_threads<G>();
   const int64_t per_block = kThreads / G;
-  return launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V>, (p.rows + per_block - 1) / per_block,
-                          kThreads, 0, s, p);
+  const int64_t blocks = (p.rows + per_block - 1) / per_block;
+  return p.dest == nullptr
+             ? launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V, false>, blocks, kThreads, 0, s, p)
+             : launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V, true>, blocks, kThreads, 0, s, p);
 }
 
 // The fewest threads that hold a row at four chunks each, or at three where that is as many or
