@@ -331,13 +331,15 @@ NVFP4_API int nvfp4_moe_combine_tokens_backward(const void* grad_out, int64_t ld
  * quotient. x bf16 or fp16 [rows, cols], any alignment and row stride ld (elements); codes
  * int8, 16-byte aligned, row stride codes_ld a multiple of 16 bytes (bytes past cols are not
  * written). A row of zeros has scale 0; a row holding an infinity or a NaN has scale NaN and
- * zero codes. row_mask (or NULL): rows with row_mask[r] < 0 are neither read nor written.
+ * zero codes. row_list (or NULL: every row): device int32 [listed], the rows to quantise, each in
+ * its place (entries outside [0, rows) are none; other rows are neither read nor written), e.g.
+ * a routing's dest for a dispatched buffer.
  * nvfp4_moe_dispatch_int8 quantises each token once and writes its codes and scale to the
  * rows dest[t * topk + j] inside [0, rows); other rows are not written.
  */
 NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
-                                  const int32_t* row_mask, void* codes, int64_t codes_ld,
-                                  float* scales, void* stream);
+                                  const int32_t* row_list, int64_t listed, void* codes,
+                                  int64_t codes_ld, float* scales, void* stream);
 NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
                                       const int32_t* dest, int topk, int64_t rows, void* codes,
                                       int64_t codes_ld, float* scales, void* stream);

@@ -322,7 +322,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.nvfp4_moe_combine_tokens_backward.argtypes = [vp, i64, vp, i64, i32, vp, vp, vp, i32,
                                                           i32, i32, i64, vp, i64, vp, vp]
         lib.nvfp4_moe_combine_tokens_backward.restype = i32
-        lib.nvfp4_quantize_int8.argtypes = [vp, i64, i32, i64, i32, vp, vp, i64, vp, vp]
+        lib.nvfp4_quantize_int8.argtypes = [vp, i64, i32, i64, i32, vp, i64, vp, i64, vp, vp]
         lib.nvfp4_quantize_int8.restype = i32
         lib.nvfp4_moe_dispatch_int8.argtypes = [vp, i32, i32, i64, i32, vp, i32, i64, vp, i64, vp,
                                                 vp]

@@ -223,7 +223,8 @@ template <typename T, int G, int V>
 cudaError_t launch_quantize_rows(const Int8QuantParams& p, cudaStream_t s) {
   constexpr int kThreads = int8_quant_threads<G>();
   const int64_t per_block = kThreads / G;
-  const int64_t blocks = (p.rows + per_block - 1) / per_block;
+  const int64_t rows = p.row_list != nullptr ? p.listed : p.rows;
+  const int64_t blocks = (rows + per_block - 1) / per_block;
   return p.dest == nullptr
              ? launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V, false>, blocks, kThreads, 0, s, p)
              : launch_dependent(&nvfp4_quantize_int8_kernel<T, G, V, true>, blocks, kThreads, 0, s, p);
@@ -246,14 +247,17 @@ cudaError_t launch_quantize_int8(const Int8QuantParams& p, cudaStream_t s) {
 }
 
 int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
-                       const int32_t* row_mask, const int32_t* dest, int topk, int64_t out_rows,
+                       const int32_t* row_list, int64_t listed, const int32_t* dest, int topk,
+                       int64_t out_rows,
                        void* codes, int64_t codes_ld, float* scales, void* stream) {
   if (dtype != NVFP4_DTYPE_BF16 && dtype != NVFP4_DTYPE_FP16)
     return fail(NVFP4_ERR_INVALID_ARGUMENT, "dtype=%d (expected NVFP4_DTYPE_BF16 or _FP16)", dtype);
   if (rows < 0 || rows > 0x7fffffff || out_rows < 0 || out_rows > 0x7fffffff || cols <= 0)
     return fail(NVFP4_ERR_BAD_SHAPE, "rows=%lld out_rows=%lld cols=%d", static_cast<long long>(rows),
                 static_cast<long long>(out_rows), cols);
-  if (rows == 0 || out_rows == 0) return NVFP4_OK;
+  if (listed < 0 || listed > 0x7fffffff)
+    return fail(NVFP4_ERR_BAD_SHAPE, "listed=%lld", static_cast<long long>(listed));
+  if (rows == 0 || out_rows == 0 || (row_list != nullptr && listed == 0)) return NVFP4_OK;
   if (x == nullptr || codes == nullptr || scales == nullptr)
     return fail(NVFP4_ERR_NULL_POINTER, "x, codes or scales is NULL");
   if (ld < cols || codes_ld < cols)
@@ -271,7 +275,8 @@ int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dt
   p.cols = cols;
   const uintptr_t at = reinterpret_cast<uintptr_t>(x);
   p.align = at % 16 == 0 && ld % 8 == 0 ? 16 : at % 4 == 0 && ld % 2 == 0 ? 4 : 2;
-  p.row_mask = row_mask;
+  p.row_list = row_list;
+  p.listed = static_cast<int32_t>(listed);
   p.dest = dest;
   p.topk = topk;
   p.out_rows = static_cast<int32_t>(out_rows);
@@ -293,11 +298,11 @@ using namespace nvfp4;
 extern "C" {
 
 NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
-                                  const int32_t* row_mask, void* codes, int64_t codes_ld,
-                                  float* scales, void* stream) {
+                                  const int32_t* row_list, int64_t listed, void* codes,
+                                  int64_t codes_ld, float* scales, void* stream) {
   g_last_error.clear();
-  return quantize_int8_impl(x, rows, cols, ld, dtype, row_mask, nullptr, 1, rows, codes, codes_ld,
-                            scales, stream);
+  return quantize_int8_impl(x, rows, cols, ld, dtype, row_list, row_list != nullptr ? listed : 0,
+                            nullptr, 1, rows, codes, codes_ld, scales, stream);
 }
 
 NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
@@ -307,7 +312,7 @@ NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64
   if (topk <= 0 || static_cast<int64_t>(tokens) * topk > (int64_t{1} << 30))
     return fail(NVFP4_ERR_BAD_SHAPE, "tokens=%d topk=%d", tokens, topk);
   if (tokens > 0 && dest == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "dest is NULL");
-  return quantize_int8_impl(x, tokens, cols, ld, dtype, nullptr, dest, topk, rows, codes, codes_ld,
+  return quantize_int8_impl(x, tokens, cols, ld, dtype, nullptr, 0, dest, topk, rows, codes, codes_ld,
                             scales, stream);
 }
 

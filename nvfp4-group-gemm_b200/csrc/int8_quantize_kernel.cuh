@@ -37,7 +37,8 @@ struct Int8QuantParams {
   int32_t rows;
   int32_t cols;
   int32_t align;         // rows of x start on 16-byte (16) or 4-byte (4) boundaries, or any (2)
-  const int32_t* row_mask;  // nullptr, or rows with row_mask[r] < 0 are left out
+  const int32_t* row_list;  // nullptr: every row; else `listed` rows (outside [0, rows): none)
+  int32_t listed;
   const int32_t* dest;   // nullptr: row r goes to row r; else to rows dest[r * topk + j]
   int32_t topk;
   int32_t out_rows;      // destinations outside [0, out_rows) are dropped
@@ -169,8 +170,9 @@ __global__ void __launch_bounds__(int8_quant_threads<G>(), 1536 / int8_quant_thr
   ptx::griddep_launch_dependents();
   const int group = threadIdx.x / G;
   const int gt = threadIdx.x % G;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + group;
-  const bool active = r < p.rows && (p.row_mask == nullptr || __ldg(p.row_mask + r) >= 0);
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + group;
+  if (!DISPATCH && p.row_list != nullptr) r = r < p.listed ? __ldg(p.row_list + r) : -1;
+  const bool active = r >= 0 && r < p.rows;
   const uint16_t* row = p.x + r * p.ld;
   const int cols = active ? p.cols : 0;
   uint32_t v[V][4];

@@ -107,32 +107,36 @@ def _check_code_outputs(codes, scales, rows: int, cols: int) -> None:
 
 
 def quantize_int8(x: torch.Tensor, codes: torch.Tensor | None = None,
-                  scales: torch.Tensor | None = None, row_mask: torch.Tensor | None = None,
+                  scales: torch.Tensor | None = None, row_list: torch.Tensor | None = None,
                   stream: torch.cuda.Stream | None = None) -> tuple:
     """Quantise the rows of ``x`` (bf16 or fp16 [rows, cols]) to int8: ``(codes, scales)`` with
     ``scales[r] = max|x[r]| / 127`` and ``codes = 127 * x / max|x[r]|`` rounded to nearest, ties
     to even (of the exact quotient), so ``x ~= codes * scales[:, None]``.
 
     A row of zeros gets scale 0; a row that holds an infinity or a NaN gets scale NaN and zero
-    codes. ``row_mask`` (int32 [rows], e.g. a routing's ``src_rows``): rows where it is negative
-    are neither read nor written. ``codes`` / ``scales`` write in place.
+    codes. ``row_list`` (1-D int32, e.g. a routing's ``dest`` for a dispatched buffer): only these
+    rows are quantised, each in its place (entries outside ``[0, rows)`` are none); the others are
+    neither read nor written. ``codes`` / ``scales`` write in place.
     """
     _check_activations(x)
     rows, cols = int(x.shape[0]), int(x.shape[1])
     _check_code_outputs(codes, scales, rows, cols)
-    if row_mask is not None and (row_mask.dtype != torch.int32 or not row_mask.is_contiguous() or
-                                 row_mask.dim() != 1 or row_mask.numel() < rows):
-        raise ValueError(f"row_mask must be a contiguous int32 tensor of >= {rows} entries")
-    s, where = _launch_on((x, codes, scales, row_mask), stream)
+    if row_list is not None and (row_list.dtype != torch.int32 or row_list.dim() != 1 or
+                                 not row_list.is_contiguous()):
+        raise ValueError("row_list must be a contiguous 1-D int32 tensor")
+    s, where = _launch_on((x, codes, scales, row_list), stream)
     with where:
         if codes is None:
             codes = empty_codes(rows, cols, x.device)
         if scales is None:
             scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+        if row_list is not None and row_list.numel() == 0:
+            return codes, scales
         lib = _native.load_library()
         _native.check(lib.nvfp4_quantize_int8(
             x.data_ptr(), rows, cols, _row_stride(x), _IN_DTYPES[x.dtype],
-            row_mask.data_ptr() if row_mask is not None else None, codes.data_ptr(),
+            row_list.data_ptr() if row_list is not None else None,
+            row_list.numel() if row_list is not None else 0, codes.data_ptr(),
             _codes_stride(codes, "codes"), scales.data_ptr(), s), lib)
     return codes, scales
 

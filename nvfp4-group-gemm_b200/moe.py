@@ -582,7 +582,7 @@ class Int8MoEBlock:
             int8_gemm_segments(self._a, self._a_scale, W.w_gate, W.s_gate, self.offsets, self.counts,
                                b2=W.w_up, b2_scale=W.s_up, out=self._h, expected_rows=T * K,
                                stream=st)
-            quantize_int8(self._h, self._a2, self._a2_scale, row_mask=self.src_rows, stream=st)
+            quantize_int8(self._h, self._a2, self._a2_scale, row_list=self.dest, stream=st)
             int8_gemm_segments(self._a2, self._a2_scale, W.w_down, W.s_down, self.offsets,
                                self.counts, out=self._y, expected_rows=T * K, stream=st)
             w = topk_weights

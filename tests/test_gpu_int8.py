@@ -110,18 +110,21 @@ def test_quantize_extreme_rows(pkg):
     assert np.all(np.abs(_np(scales)[ok] - ws[ok]) <= U * ws[ok] + 2.0 ** -149)
 
 
-def test_quantize_strided_input_mask_and_untouched_bytes(pkg):
+def test_quantize_strided_input_listed_rows_and_untouched_bytes(pkg):
     base = torch.randn((33, 301), generator=torch.Generator().manual_seed(4)).to(torch.float16).cuda()
     x = base[:, 5:5 + 203]  # rows 301 elements apart, odd start
     buf = torch.full((33, 256), 77, dtype=torch.int8, device="cuda")
     scales = torch.full((33,), -1.0, device="cuda")
-    mask = torch.zeros(40, dtype=torch.int32)
-    mask[::3] = -1
-    pkg.quantize_int8(x, codes=buf[:, :203], scales=scales, row_mask=mask.cuda())
+    rows = torch.tensor([4, -1, 32, 0, 33, 4, 17, 2 ** 31 - 1, -5], dtype=torch.int32, device="cuda")
+    pkg.quantize_int8(x, codes=buf[:, :203], scales=scales, row_list=rows)
     want, ws = O.quantize_int8(_np(x))
-    keep = (mask[:33] >= 0).numpy()
+    keep = np.zeros(33, dtype=bool)
+    keep[[4, 32, 0, 17]] = True
     assert np.array_equal(buf.cpu().numpy()[keep, :203], want[keep])
+    assert np.all(np.abs(_np(scales)[keep] - ws[keep]) <= U * ws[keep])
     assert np.all(buf.cpu().numpy()[~keep] == 77) and np.all(buf.cpu().numpy()[:, 203:] == 77)
+    assert np.all(_np(scales)[~keep] == -1.0)
+    pkg.quantize_int8(x, codes=buf[:, :203], scales=scales, row_list=rows[:0])  # none
     assert np.all(_np(scales)[~keep] == -1.0)
 
 

@@ -154,7 +154,7 @@ def test_operators_on_two_streams_at_once(pkg):
         a, sa = pkg.moe.dispatch_int8(x, r, stream=st)
         h = pkg.int8_gemm_segments(a, sa, W.w_gate, W.s_gate, off, cnt, b2=W.w_up, b2_scale=W.s_up,
                                    stream=st)
-        a2, sa2 = pkg.quantize_int8(h, row_mask=r.src_rows, stream=st)
+        a2, sa2 = pkg.quantize_int8(h, row_list=r.dest, stream=st)
         y = pkg.int8_gemm_segments(a2, sa2, W.w_down, W.s_down, off, cnt, stream=st)
         return pkg.moe.combine_tokens(y, r, w, stream=st)
 

@@ -48,8 +48,9 @@ def test_product_struct_layout(pkg):
 def test_quantiser_statuses(pkg):
     lib = pkg.load_library()
 
-    def call(x=0x1000, rows=4, cols=33, ld=33, dtype=0, mask=None, codes=0x2000, codes_ld=48, scales=0x3000):
-        return lib.nvfp4_quantize_int8(x, rows, cols, ld, dtype, mask, codes, codes_ld, scales, None)
+    def call(x=0x1000, rows=4, cols=33, ld=33, dtype=0, listed=None, n=0, codes=0x2000, codes_ld=48,
+             scales=0x3000):
+        return lib.nvfp4_quantize_int8(x, rows, cols, ld, dtype, listed, n, codes, codes_ld, scales, None)
 
     assert call(dtype=2) == 1 and call(dtype=-1) == 1
     assert call(cols=0) == 2 and call(rows=-1) == 2 and call(rows=2 ** 31) == 2
@@ -57,6 +58,7 @@ def test_quantiser_statuses(pkg):
     assert call(ld=32) == 1 and call(codes_ld=32) == 1
     assert call(codes=0x2008) == 3 and call(codes_ld=40) == 3
     assert call(rows=0) == 0
+    assert call(listed=0x4000, n=0) == 0 and call(listed=0x4000, n=-1) == 2 and call(listed=0x4000, n=2 ** 31) == 2
 
     def dispatch(tokens=4, topk=2, dest=0x4000, rows=128, cols=33):
         return lib.nvfp4_moe_dispatch_int8(0x1000, tokens, cols, 33, 0, dest, topk, rows, 0x2000, 48, 0x3000, None)
