@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import numpy as np
@@ -196,6 +197,12 @@ class Int8Product(ctypes.Structure):
     ]
 
 
+# The same record packed in one step (its fields in order, 0 for NULL): the bytes are passed as
+# they are, at a third of the time that filling the ctypes structure takes.
+pack_int8_product = struct.Struct("<10Q5q4i").pack
+assert len(pack_int8_product(*[0] * 19)) == ctypes.sizeof(Int8Product)
+
+
 # Nvfp4Group as a numpy structured dtype, so that a whole group table is
 # filled with a few vectorised column assignments instead of per-field ctypes calls.
 GROUP_DTYPE = np.dtype(
@@ -327,7 +334,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.nvfp4_moe_dispatch_int8.argtypes = [vp, i32, i32, i64, i32, vp, i32, i64, vp, i64, vp,
                                                 vp]
         lib.nvfp4_moe_dispatch_int8.restype = i32
-        lib.nvfp4_int8_gemm.argtypes = [ctypes.POINTER(Int8Product), vp]
+        lib.nvfp4_int8_gemm.argtypes = [vp, vp]
         lib.nvfp4_int8_gemm.restype = i32
         lib.nvfp4_int8_check.argtypes = [vp, ctypes.POINTER(ctypes.c_uint)]
         lib.nvfp4_int8_check.restype = i32

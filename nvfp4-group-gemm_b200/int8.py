@@ -12,7 +12,6 @@ in any CUDA graphs. The reference has no 8-bit form of its product.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -23,28 +22,33 @@ _IN_DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F
 _OUT_DTYPES = {**_IN_DTYPES, torch.float32: _native.DTYPE_FP32}
 
 
-_HERE = contextlib.nullcontext()
-
-
 def _launch_on(tensors, stream: torch.cuda.Stream | None) -> tuple:
     """``(raw stream, context)`` of a call on ``tensors`` (None entries left out; the first gives
-    the device, the others must be on it). The context makes device and stream current, so that
-    what is allocated inside belongs to the stream. Tensors used on another stream than the
-    current one are recorded there, so that freeing them early does not hand their memory out
-    while the call runs."""
+    the device, the others must be on it). The context, None where nothing has to change, makes
+    device and stream current, so that what is allocated inside belongs to the stream. Tensors
+    used on another stream than the current one are recorded there, so that freeing them early
+    does not hand their memory out while the call runs."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index or index < 0:
             raise ValueError("all tensors must be CUDA tensors on one device")
     raw = torch._C._cuda_getCurrentRawStream(index)
     if stream is None or (stream.cuda_stream == raw and stream.device.index == index):
-        return raw, _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+        return raw, None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
     if stream.device.index != index:
         raise ValueError(f"stream is on {stream.device}, the tensors are on cuda:{index}")
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
     return stream.cuda_stream, torch.cuda.stream(stream)
+
+
+def _within(where, call, *args):
+    """``call(*args)`` inside the context of :func:`_launch_on`."""
+    if where is None:
+        return call(*args)
+    with where:
+        return call(*args)
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -69,10 +73,8 @@ def _check_activations(x: torch.Tensor) -> None:
 
 def _codes_stride(t: torch.Tensor, name: str) -> int:
     """Bytes between the rows of an int8 code matrix [rows, k] (checked)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int8:
-        raise ValueError(f"{name} must be a CUDA int8 tensor")
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be 2-D")
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int8 or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D CUDA int8 tensor")
     rows, cols = t.shape
     ld, inner = t.stride()
     if cols < 1 or (inner != 1 and cols != 1):
@@ -86,8 +88,8 @@ def _codes_stride(t: torch.Tensor, name: str) -> int:
 
 
 def _check_scale(t: torch.Tensor, shape: tuple, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or \
-            t.shape != shape or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != shape or \
+            not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous CUDA float32 tensor of shape {list(shape)}")
 
 
@@ -124,30 +126,26 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor | None = None,
     if row_list is not None and (row_list.dtype != torch.int32 or row_list.dim() != 1 or
                                  not row_list.is_contiguous()):
         raise ValueError("row_list must be a contiguous 1-D int32 tensor")
-    s, where = _launch_on((x, codes, scales, row_list), stream)
-    with where:
-        if codes is None:
-            codes = empty_codes(rows, cols, x.device)
-        if scales is None:
-            scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-        if row_list is not None and row_list.numel() == 0:
+    raw, where = _launch_on((x, codes, scales, row_list), stream)
+    return _within(where, _quantize, x, rows, cols, codes, scales, row_list, raw)
+
+
+def _quantize(x, rows, cols, codes, scales, row_list, raw):
+    if codes is None:
+        codes = empty_codes(rows, cols, x.device)
+    if scales is None:
+        scales = x.new_empty(rows, dtype=torch.float32)
+    listed = 0
+    if row_list is not None:
+        listed = row_list.numel()
+        if listed == 0:
             return codes, scales
-        lib = _native.load_library()
-        _native.check(lib.nvfp4_quantize_int8(
-            x.data_ptr(), rows, cols, _row_stride(x), _IN_DTYPES[x.dtype],
-            row_list.data_ptr() if row_list is not None else None,
-            row_list.numel() if row_list is not None else 0, codes.data_ptr(),
-            _codes_stride(codes, "codes"), scales.data_ptr(), s), lib)
+    lib = _native.load_library()
+    _native.check(lib.nvfp4_quantize_int8(
+        x.data_ptr(), rows, cols, _row_stride(x), _IN_DTYPES[x.dtype],
+        row_list.data_ptr() if listed else None, listed, codes.data_ptr(),
+        _codes_stride(codes, "codes"), scales.data_ptr(), raw), lib)
     return codes, scales
-
-
-def _out_for(out, out_dtype, rows: int, n: int, like) -> torch.Tensor:
-    if out is None:
-        dtype = torch.bfloat16 if out_dtype is None else out_dtype
-        if dtype not in _OUT_DTYPES:
-            raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {dtype}")
-        return like.new_empty((rows, n), dtype=dtype)
-    return out
 
 
 def _check_out(out, out_dtype, rows: int, n: int) -> None:
@@ -162,18 +160,26 @@ def _check_out(out, out_dtype, rows: int, n: int) -> None:
         raise ValueError(f"out is {out.dtype}, out_dtype is {out_dtype}")
 
 
-def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, n, k, experts, offsets,
-             counts, expected_rows, stream) -> None:
+def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, out_dtype, n, k, experts,
+             offsets, counts, expected_rows, raw):
     rows = a.shape[0]
-    p = _native.Int8Product(  # positional: the fields in their order
-        a.data_ptr(), b.data_ptr(), b2.data_ptr() if b2 is not None else None, a_scale.data_ptr(),
-        b_scale.data_ptr(), b2_scale.data_ptr() if b2 is not None else None,
-        bias.data_ptr() if bias is not None else None, out.data_ptr(),
-        offsets.data_ptr() if offsets is not None else None,
-        counts.data_ptr() if counts is not None else None, rows, lda, ldb, _row_stride(out),
-        expected_rows, n, k, experts, _OUT_DTYPES[out.dtype])
+    if out is None:
+        dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        if dtype not in _OUT_DTYPES:
+            raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {dtype}")
+        out, ldo = a.new_empty((rows, n), dtype=dtype), n
+    else:
+        dtype, ldo = out.dtype, _row_stride(out)
+    product = _native.pack_int8_product(
+        a.data_ptr(), b.data_ptr(), b2.data_ptr() if b2 is not None else 0, a_scale.data_ptr(),
+        b_scale.data_ptr(), b2_scale.data_ptr() if b2 is not None else 0,
+        bias.data_ptr() if bias is not None else 0, out.data_ptr(),
+        offsets.data_ptr() if offsets is not None else 0,
+        counts.data_ptr() if counts is not None else 0, rows, lda, ldb, ldo, expected_rows, n, k,
+        experts, _OUT_DTYPES[dtype])
     lib = _native.load_library()
-    _native.check(lib.nvfp4_int8_gemm(ctypes.byref(p), stream), lib)
+    _native.check(lib.nvfp4_int8_gemm(product, raw), lib)
+    return out
 
 
 def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -199,11 +205,9 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     if bias is not None:
         _check_scale(bias, (n,), "bias")
     _check_out(out, out_dtype, m, n)
-    s, where = _launch_on((a, a_scale, b, b_scale, bias, out), stream)
-    with where:
-        out = _out_for(out, out_dtype, m, n, a)
-        _product(a, lda, a_scale, b, ldb, b_scale, None, None, bias, out, n, k, 1, None, None, 0, s)
-    return out
+    raw, where = _launch_on((a, a_scale, b, b_scale, bias, out), stream)
+    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, None, None, bias, out, out_dtype,
+                   n, k, 1, None, None, 0, raw)
 
 
 def _expert_weights(b: torch.Tensor, b_scale: torch.Tensor, k: int, name: str) -> int:
@@ -259,12 +263,10 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
         if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < experts:
             raise ValueError(f"{name} must be a contiguous CUDA int32 tensor of >= {experts} entries")
     _check_out(out, out_dtype, rows, n)
-    s, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out), stream)
-    with where:
-        out = _out_for(out, out_dtype, rows, n, a)
-        _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out, n, k, experts,
-                 seg_offsets, seg_counts, int(expected_rows), s)
-    return out
+    raw, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out),
+                            stream)
+    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out, out_dtype,
+                   n, k, experts, seg_offsets, seg_counts, int(expected_rows), raw)
 
 
 def check_int8_errors(device: torch.device | int | None = None,

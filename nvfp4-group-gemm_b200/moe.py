@@ -31,8 +31,8 @@ import torch
 from . import _native
 from .interface import grouped_gemm_table
 from .layout import blocked_sf_bytes
-from .int8 import _check_activations, _check_code_outputs, _codes_stride, _launch_on, _row_stride
-from .int8 import check_int8_errors, empty_codes, int8_gemm_segments, quantize_int8
+from .int8 import (_check_activations, _check_code_outputs, _codes_stride, _launch_on, _row_stride,
+                   _within, check_int8_errors, empty_codes, int8_gemm_segments, quantize_int8)
 from .quantize import _DTYPES, global_scale_for, quantize
 from .token_sort import (combine_tokens, combine_tokens_backward, dispatch_tokens,  # noqa: F401
                          dispatch_tokens_backward)
@@ -155,17 +155,20 @@ def dispatch_int8(x: torch.Tensor, routing: Routing, codes: torch.Tensor | None 
         raise ValueError(f"routing.dest must be contiguous int32 with "
                          f"{routing.tokens * routing.topk} entries")
     _check_code_outputs(codes, scales, rows, cols)
-    s, where = _launch_on((x, dest, codes, scales), stream)
-    with where:
-        if codes is None:
-            codes = empty_codes(rows, cols, x.device)
-        if scales is None:
-            scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-        lib = _native.load_library()
-        _native.check(lib.nvfp4_moe_dispatch_int8(
-            x.data_ptr(), routing.tokens, cols, _row_stride(x), _DTYPES[x.dtype], dest.data_ptr(),
-            routing.topk, rows, codes.data_ptr(), _codes_stride(codes, "codes"),
-            scales.data_ptr(), s), lib)
+    raw, where = _launch_on((x, dest, codes, scales), stream)
+    return _within(where, _dispatch_int8, x, routing, rows, cols, codes, scales, raw)
+
+
+def _dispatch_int8(x, routing, rows, cols, codes, scales, raw):
+    if codes is None:
+        codes = empty_codes(rows, cols, x.device)
+    if scales is None:
+        scales = x.new_empty(rows, dtype=torch.float32)
+    lib = _native.load_library()
+    _native.check(lib.nvfp4_moe_dispatch_int8(
+        x.data_ptr(), routing.tokens, cols, _row_stride(x), _DTYPES[x.dtype], routing.dest.data_ptr(),
+        routing.topk, rows, codes.data_ptr(), _codes_stride(codes, "codes"), scales.data_ptr(), raw),
+        lib)
     return codes, scales
 
 

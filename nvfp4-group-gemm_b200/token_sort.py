@@ -21,12 +21,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .int8 import _OUT_DTYPES, _launch_on
+from .int8 import _OUT_DTYPES, _launch_on, _within
 
 
 def _check_routing(routing) -> tuple:
     """``(tokens, topk, rows, dest, src_rows)`` of a Routing, checked against one another."""
-    tokens, topk, rows = int(routing.tokens), int(routing.topk), int(routing.rows)
+    tokens, topk, rows = routing.tokens, routing.topk, routing.rows
     dest, src = routing.dest, routing.src_rows
     if dest.dtype != torch.int32 or dest.numel() < tokens * topk or not dest.is_contiguous():
         raise ValueError(f"routing.dest must be contiguous int32 with {tokens * topk} entries")
@@ -36,10 +36,10 @@ def _check_routing(routing) -> tuple:
 
 
 def _check_rows(t: torch.Tensor, rows: int, name: str, cols: int | None = None) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _OUT_DTYPES:
-        raise ValueError(f"{name} must be a CUDA bf16, fp16 or fp32 tensor")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or \
-            (cols is not None and t.shape[1] != cols):
+    if not isinstance(t, torch.Tensor) or t.dtype not in _OUT_DTYPES or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D CUDA bf16, fp16 or fp32 tensor")
+    have = t.shape
+    if have[0] != rows or have[1] < 1 or (cols is not None and have[1] != cols):
         want = f"[{rows}, {'cols' if cols is None else cols}]"
         raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
 
@@ -116,9 +116,8 @@ def _check_weights(weights, tokens, topk):
 def _dispatch(x, routing, stream):
     tokens, topk, rows, dest, src = _check_routing(routing)
     _check_rows(x, tokens, "x")
-    s, where = _launch_on((x, dest, src), stream)
-    with where:
-        return _launch_dispatch(x, dest, src, (tokens, topk, rows), s)
+    raw, where = _launch_on((x, dest, src), stream)
+    return _within(where, _launch_dispatch, x, dest, src, (tokens, topk, rows), raw)
 
 
 def _combine(y, routing, weights, stream):
@@ -126,9 +125,8 @@ def _combine(y, routing, weights, stream):
     _check_rows(y, rows, "y")
     if weights is not None:
         _check_weights(weights, tokens, topk)
-    s, where = _launch_on((y, dest, weights), stream)
-    with where:
-        return _launch_combine(y, dest, weights, (tokens, topk, rows), s)
+    raw, where = _launch_on((y, dest, weights), stream)
+    return _within(where, _launch_combine, y, dest, weights, (tokens, topk, rows), raw)
 
 
 def dispatch_tokens_backward(grad_y: torch.Tensor, routing,
@@ -158,10 +156,9 @@ def combine_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor | None, rout
     if weights is not None:
         _check_weights(weights, tokens, topk)
     y = y if want_weights else None
-    s, where = _launch_on((grad_out, dest, src, weights, y), stream)
-    with where:
-        return _launch_combine_backward(grad_out, y, dest, src, weights, (tokens, topk, rows), want_y,
-                                        s)
+    raw, where = _launch_on((grad_out, dest, src, weights, y), stream)
+    return _within(where, _launch_combine_backward, grad_out, y, dest, src, weights,
+                   (tokens, topk, rows), want_y, raw)
 
 
 class _Kept:
@@ -178,7 +175,7 @@ class _DispatchTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, routing):
         dest, src = routing.dest, routing.src_rows
-        ctx.sizes = (int(routing.tokens), int(routing.topk), int(routing.rows))
+        ctx.sizes = routing.tokens, routing.topk, routing.rows
         ctx.save_for_backward(dest, src)
         return _dispatch(x, routing, None)
 
@@ -205,7 +202,7 @@ class _CombineTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, routing):
         want_w = weights is not None and ctx.needs_input_grad[1]
-        ctx.sizes = (int(routing.tokens), int(routing.topk), int(routing.rows))
+        ctx.sizes = routing.tokens, routing.topk, routing.rows
         ctx.save_for_backward(routing.dest, routing.src_rows, weights, y if want_w else None)
         return _combine(y, routing, weights, None)
 
