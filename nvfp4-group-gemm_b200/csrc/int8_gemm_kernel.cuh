@@ -56,62 +56,37 @@ struct Int8GemmParams {
   int32_t ktiles;
   int32_t num_experts;
   int32_t out_dtype;
-  int32_t out_vec;  // rows of out start on 16-byte boundaries
 };
 
 // Outputs of 32 channels (one per lane) x M tokens: y[i] is row i's, the first `count` rows are
-// stored. Where rows start on 16-byte boundaries and all 32 channels exist, the block is turned
-// in shared memory (buf, 32 M elements) and stored in 16-byte pieces, else element by element.
-// (Two-byte stores alone, 64 bytes per instruction, took 6.8 us for a tile of 128 channels x
-// 256 tokens, longer than its MMAs at K = 1536.)
+// stored, a row's 32 channels at a time. (Turned in shared memory first and stored in 16-byte
+// pieces, with this as the path of unaligned rows, 65,536 expert rows at N 4096, K 1536 took
+// 370 - 390 us instead of 325.)
 template <typename T, int M>
 __device__ __forceinline__ void int8_store_rows_as(T* out, int64_t ldo, const float (&y)[M],
-                                                   int count, int channels, bool vec,
-                                                   uint8_t* buf, int lane) {
-  auto as_out = [](float v) {
-    if constexpr (sizeof(T) == 4) return v;
-    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
-    else return __float2bfloat16_rn(v);
-  };
-  if (vec && channels >= 32) {
-    constexpr int kPieces = 2 * sizeof(T);  // 16-byte pieces of a row
-    constexpr int kRows = 32 / kPieces;     // rows per store instruction
-    T* turn = reinterpret_cast<T*>(buf);
-    __syncwarp();  // the previous block is stored
+                                                   int count) {
 #pragma unroll
-    for (int i = 0; i < M; ++i) turn[32 * i + lane] = as_out(y[i]);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < M; i += kRows) {
-      const int r = i + lane / kPieces;
-      if (r < count)
-        *reinterpret_cast<uint4*>(out + r * ldo + lane % kPieces * (32 / kPieces)) =
-            *reinterpret_cast<const uint4*>(buf + 16 * (kPieces * r + lane % kPieces));
+  for (int i = 0; i < M; ++i) {
+    if (i < count) {
+      if constexpr (sizeof(T) == 4) *out = y[i];
+      else if constexpr (std::is_same<T, __half>::value) *out = __float2half_rn(y[i]);
+      else *out = __float2bfloat16_rn(y[i]);
     }
-  } else if (lane < channels) {
-    out += lane;
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-      if (i < count) *out = as_out(y[i]);
-      out += ldo;
-    }
+    out += ldo;
   }
 }
-// row0: first token row; n0: the lanes' first channel.
+// row0: first token row; n: this lane's channel (nothing is stored past the last one).
 template <int M>
-__device__ __forceinline__ void int8_store_rows(const Int8GemmParams& p, int64_t row0, int n0,
-                                                const float (&y)[M], int count, uint8_t* buf,
-                                                int lane) {
-  const int64_t at = row0 * p.ldo + n0;
-  const int channels = p.n - n0;
-  const bool vec = p.out_vec != 0;
+__device__ __forceinline__ void int8_store_rows(const Int8GemmParams& p, int64_t row0, int n,
+                                                const float (&y)[M], int count) {
+  if (n >= p.n) return;
+  const int64_t at = row0 * p.ldo + n;
   if (p.out_dtype == kInt8OutBf16)
-    int8_store_rows_as(static_cast<__nv_bfloat16*>(p.out) + at, p.ldo, y, count, channels, vec, buf,
-                       lane);
+    int8_store_rows_as(static_cast<__nv_bfloat16*>(p.out) + at, p.ldo, y, count);
   else if (p.out_dtype == kInt8OutFp16)
-    int8_store_rows_as(static_cast<__half*>(p.out) + at, p.ldo, y, count, channels, vec, buf, lane);
+    int8_store_rows_as(static_cast<__half*>(p.out) + at, p.ldo, y, count);
   else
-    int8_store_rows_as(static_cast<float*>(p.out) + at, p.ldo, y, count, channels, vec, buf, lane);
+    int8_store_rows_as(static_cast<float*>(p.out) + at, p.ldo, y, count);
 }
 
 __device__ __forceinline__ float int8_silu_mul(float g, float u) {
@@ -201,8 +176,7 @@ struct Int8Config {
   static constexpr int kWBytes = 128 * kInt8StageK;
   static constexpr int kXBytes = TN * kInt8StageK;
   static constexpr int kStageBytes = kSets * kWBytes + kXBytes;
-  static constexpr int kTurnBytes = 16 * 128;  // a warp's block of 16 tokens x 32 channels
-  static constexpr int kFixedBytes = 1024 + kInt8SegBytes + kEpiWarps * kTurnBytes + 512;
+  static constexpr int kFixedBytes = 1024 + kInt8SegBytes + 512;
   static constexpr int kFit = (232448 - kFixedBytes) / kStageBytes;
   static constexpr int kStages = kFit > 12 ? 12 : kFit;
   static constexpr int kSmemBytes = kFixedBytes + kStages * kStageBytes;
@@ -224,8 +198,7 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* turn = smem + kStages * Cfg::kStageBytes;
-  int32_t* seg_row = reinterpret_cast<int32_t*>(turn + Cfg::kEpiWarps * Cfg::kTurnBytes);
+  int32_t* seg_row = reinterpret_cast<int32_t*>(smem + kStages * Cfg::kStageBytes);
   int32_t* seg_cnt = seg_row + kInt8MaxExperts;
   int32_t* seg_end = seg_cnt + kInt8MaxExperts;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(seg_end + kInt8MaxExperts);
@@ -433,8 +406,7 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
         for (int i = 0; i < 16; ++i)
           y[i] = value(static_cast<int32_t>(v[i]), GATED ? static_cast<int32_t>(u[i]) : 0,
                        __shfl_sync(0xffffffffu, as[c / 32], (c + i) & 31));
-        int8_store_rows(p, static_cast<int64_t>(t.row) + tok0 + c, n - lane, y, toks - c,
-                        turn + (warp - kEpilogueWarp0) * Cfg::kTurnBytes, lane);
+        int8_store_rows(p, static_cast<int64_t>(t.row) + tok0 + c, n, y, toks - c);
       }
       ptx::tcgen05_fence_before_sync();
       __syncwarp();

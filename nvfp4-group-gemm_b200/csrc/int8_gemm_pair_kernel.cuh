@@ -37,13 +37,12 @@ struct Int8PairConfig {
   static constexpr int kWBytes = 128 * kInt8StageK;
   static constexpr int kXBytes = kInt8PairTokens / 2 * kInt8StageK;
   static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kStages = GATED ? 5 : 6;
+  static constexpr int kStages = 6;
   // Exchange of two warps: two buffers of 2 directions x 8 tokens x 32 channels.
   static constexpr int kPairBytes = 2 * 2 * 8 * 32 * 4;
   static constexpr int kExchangeBytes = GATED ? kInt8PairEpiWarps / 2 * kPairBytes : 0;
-  static constexpr int kTurnBytes = 16 * 128;  // a warp's block of 16 tokens x 32 channels
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kExchangeBytes +
-                                    kInt8PairEpiWarps * kTurnBytes + kInt8SegBytes + 512;
+  static constexpr int kSmemBytes =
+      1024 + kStages * kStageBytes + kExchangeBytes + kInt8SegBytes + 512;
   static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory per CTA");
 };
 
@@ -60,8 +59,8 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* exchange = reinterpret_cast<float*>(smem + kStages * Cfg::kStageBytes);
-  uint8_t* turn = smem + kStages * Cfg::kStageBytes + Cfg::kExchangeBytes;
-  int32_t* seg_row = reinterpret_cast<int32_t*>(turn + kInt8PairEpiWarps * Cfg::kTurnBytes);
+  int32_t* seg_row = reinterpret_cast<int32_t*>(smem + kStages * Cfg::kStageBytes +
+                                                Cfg::kExchangeBytes);
   int32_t* seg_cnt = seg_row + kInt8MaxExperts;
   int32_t* seg_end = seg_cnt + kInt8MaxExperts;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(seg_end + kInt8MaxExperts);
@@ -228,7 +227,6 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
     const bool up = GATED && quarter >= 2;
     const int group = GATED ? quarter & 1 : quarter;  // 32 channels of the CTA's
     float* swap = exchange + (2 * odd + group) * (Cfg::kPairBytes / 4) + lane;
-    uint8_t* buf = turn + (warp - kEpilogueWarp0) * Cfg::kTurnBytes;
     uint32_t full_parity = 0;
     uint32_t local = 0;
     uint32_t swaps = 0;
@@ -272,7 +270,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
         if (!GATED) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = __fadd_rn(y[i], bias);
-          int8_store_rows(p, static_cast<int64_t>(t.row) + tok, n - lane, y, t.rows - tok, buf, lane);
+          int8_store_rows(p, static_cast<int64_t>(t.row) + tok, n, y, t.rows - tok);
         } else {
           // The gate warp finishes tokens 0-7 of the chunk, the up warp tokens 8-15.
           float* to = swap + (2 * (swaps & 1u) + (up ? 1 : 0)) * 256;
@@ -295,8 +293,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
             z[i] = up ? int8_silu_mul(other, y[8 + i]) : int8_silu_mul(y[i], other);
           }
           const int first8 = tok + (up ? 8 : 0);
-          int8_store_rows(p, static_cast<int64_t>(t.row) + first8, n - lane, z, t.rows - first8, buf,
-                          lane);
+          int8_store_rows(p, static_cast<int64_t>(t.row) + first8, n, z, t.rows - first8);
         }
       }
       ptx::tcgen05_fence_before_sync();

@@ -370,7 +370,6 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
   p.out_dtype = g->out_dtype == NVFP4_DTYPE_BF16   ? kInt8OutBf16
                 : g->out_dtype == NVFP4_DTYPE_FP16 ? kInt8OutFp16
                                                    : kInt8OutFp32;
-  p.out_vec = aligned16(g->out) && g->ldo * (p.out_dtype == kInt8OutFp32 ? 4 : 2) % 16 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return gated ? choose_int8<true>(g, p, *ds, s) : choose_int8<false>(g, p, *ds, s);
 }

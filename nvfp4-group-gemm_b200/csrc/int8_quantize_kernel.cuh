@@ -221,18 +221,18 @@ __global__ void __launch_bounds__(int8_quant_threads<G>(), 1536 / int8_quant_thr
   for (int u = 0; u < V; ++u) q[u] = int8_codes8<T>(v[u], k);
   // Every destination of the row (row index, or -1), four looked up at a time.
   auto for_rows = [&](auto&& store) {
-    if (!DISPATCH) {
+    if constexpr (!DISPATCH) {
       store(static_cast<int32_t>(r));
-      return;
-    }
-    for (int j0 = 0; j0 < p.topk; j0 += 4) {
-      int32_t d[4];
+    } else {
+      for (int j0 = 0; j0 < p.topk; j0 += 4) {
+        int32_t d[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        d[j] = j0 + j < p.topk ? __ldg(p.dest + r * p.topk + j0 + j) : -1;
+        for (int j = 0; j < 4; ++j)
+          d[j] = j0 + j < p.topk ? __ldg(p.dest + r * p.topk + j0 + j) : -1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (d[j] >= 0 && d[j] < p.out_rows) store(d[j]);
+        for (int j = 0; j < 4; ++j)
+          if (d[j] >= 0 && d[j] < p.out_rows) store(d[j]);
+      }
     }
   };
   for_rows([&](int32_t d) {
