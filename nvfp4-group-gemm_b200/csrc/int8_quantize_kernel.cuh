@@ -155,9 +155,10 @@ __device__ __forceinline__ void int8_store_chunk(int8_t* row, int c0, int cols, 
 }
 
 // G threads on a row, each with V chunks of it in registers; blocks of one row, or of 128 threads
-// where fewer hold one. DISPATCH: a row goes to the rows dest names, else to its own. Small blocks start and end without waiting for one another: 69,632 rows
-// of 4096 columns took 149 us (0.88 of the measured copy rate) in blocks of 128, 159 in blocks of
-// 256, and 198 with the exact check on every element.
+// where fewer hold one. DISPATCH: a row goes to the rows dest names, else to its own. Small blocks
+// start and end without waiting for one another: 69,632 rows of 4096 columns took 149 us (0.88 of
+// the measured copy rate) in blocks of 128, 159 in blocks of 256, and 198 with the exact check on
+// every element.
 template <int G>
 __host__ __device__ constexpr int int8_quant_threads() { return G < 128 ? 128 : G; }
 

@@ -206,8 +206,8 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
         _check_scale(bias, (n,), "bias")
     _check_out(out, out_dtype, m, n)
     raw, where = _launch_on((a, a_scale, b, b_scale, bias, out), stream)
-    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, None, None, bias, out, out_dtype,
-                   n, k, 1, None, None, 0, raw)
+    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, None, None, bias, out,
+                   out_dtype, n, k, 1, None, None, 0, raw)
 
 
 def _expert_weights(b: torch.Tensor, b_scale: torch.Tensor, k: int, name: str) -> int:
@@ -242,8 +242,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     all of them are left as they were (undefined where ``out`` is allocated here). A segment
     outside the slab is skipped and :func:`check_int8_errors` raises; segments that share rows
     are not supported (their rows hold either result; segments past the slab's number of rows in
-    all may be skipped and reported). ``expected_rows`` (the host's estimate of all segments' rows, e.g. tokens
-    x top-k) picks the tile shape only.
+    all may be skipped and reported). ``expected_rows`` (the host's estimate of all segments'
+    rows, e.g. tokens x top-k) picks the tile shape only.
     """
     lda = _codes_stride(a, "a")
     rows, k = int(a.shape[0]), int(a.shape[1])
@@ -265,8 +265,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     _check_out(out, out_dtype, rows, n)
     raw, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out),
                             stream)
-    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out, out_dtype,
-                   n, k, experts, seg_offsets, seg_counts, int(expected_rows), raw)
+    return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out,
+                   out_dtype, n, k, experts, seg_offsets, seg_counts, int(expected_rows), raw)
 
 
 def check_int8_errors(device: torch.device | int | None = None,

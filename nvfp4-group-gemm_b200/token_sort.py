@@ -6,7 +6,8 @@
     out = combine_tokens(rows, r, topk_weights)  # [tokens, H]
 
 bf16, fp16 and fp32, any width and row stride, differentiable in ``x``, the rows and the
-weights (with weights: once). Sums are fp32 in slot order, rounded once: results do not depend on timing.
+weights (with weights: once). Sums are fp32 in slot order, rounded once: results do not depend on
+timing.
 The ``*_backward`` functions are the gradients by themselves, for training loops that do not go
 through autograd.
 
