@@ -56,6 +56,8 @@ struct Int8GemmParams {
   int32_t ktiles;
   int32_t num_experts;
   int32_t out_dtype;
+  int32_t pair_rows;  // CTA pairs: most tokens of a tile, a multiple of 32 from 64 to 256
+  uint32_t pair_inv;  // and 2^32 / (pair_rows / 32), rounded up
 };
 
 // Outputs of 32 channels (one per lane) x M tokens: y[i] is row i's, the first `count` rows are
@@ -93,11 +95,28 @@ __device__ __forceinline__ float int8_silu_mul(float g, float u) {
   return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
+// Most token rows of a tile, and the tiles that hold `count` rows. Of CTA pairs these rows are the
+// host's choice: a multiplication instead of the division that every warp would wait for per tile
+// (exact: inv is off by less than 8 / 2^32, the dividend is below 2^27).
+template <int ROWS>
+struct Int8FixedRows {
+  static constexpr int most = ROWS;
+  __device__ __forceinline__ int tiles(int count) const { return (count + ROWS - 1) / ROWS; }
+};
+struct Int8PairRows {
+  int most;
+  uint32_t inv;
+  __device__ __forceinline__ int tiles(int count) const {
+    return static_cast<int>(__umulhi((static_cast<uint32_t>(count) + most - 1) / 32, inv));
+  }
+};
+
 // Segments of the launch in shared memory: first row, rows, and the end of each expert's tile
 // range. Warp-wide; a segment outside the slab is skipped and reported, and so is one with which
 // the segments hold more rows than the slab (they share some), so that the tiles stay within
 // the host's bound.
-__device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, int tile_rows,
+template <typename Rows>
+__device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, Rows tile_rows,
                                                     int n_tiles, int32_t* seg_row,
                                                     int32_t* seg_cnt, int32_t* seg_end, int lane) {
   int32_t carry = 0;
@@ -128,7 +147,7 @@ __device__ __forceinline__ void int8_stage_segments(const Int8GemmParams& p, int
       off = cnt = 0;
     }
     rows_before += __shfl_sync(0xffffffffu, sum, 31);
-    int32_t v = (cnt + tile_rows - 1) / tile_rows * n_tiles;
+    int32_t v = tile_rows.tiles(cnt) * n_tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int32_t t = __shfl_up_sync(0xffffffffu, v, d);
@@ -148,9 +167,9 @@ struct Int8Tile {
 };
 
 // Tile `tile` of the launch. BALANCED: an expert's tiles have equal rows (a multiple of 32, at
-// most tile_rows), the last one the remainder.
-template <bool BALANCED>
-__device__ __forceinline__ Int8Tile int8_find_tile(int tile, int tile_rows, int n_tiles,
+// tile_rows.most), the last one the remainder.
+template <bool BALANCED, typename Rows>
+__device__ __forceinline__ Int8Tile int8_find_tile(int tile, Rows tile_rows, int n_tiles,
                                                    int num_experts, const int32_t* seg_row,
                                                    const int32_t* seg_cnt,
                                                    const int32_t* seg_end) {
@@ -161,10 +180,10 @@ __device__ __forceinline__ Int8Tile int8_find_tile(int tile, int tile_rows, int 
     else lo = mid + 1;
   }
   const int cnt = seg_cnt[lo];
-  const int tiles_m = (cnt + tile_rows - 1) / tile_rows;
+  const int tiles_m = tile_rows.tiles(cnt);
   const int local = tile - (seg_end[lo] - tiles_m * n_tiles);
   const int mt = local % tiles_m;
-  const int rows = BALANCED ? ((cnt + tiles_m - 1) / tiles_m + 31) / 32 * 32 : tile_rows;
+  const int rows = BALANCED ? ((cnt + tiles_m - 1) / tiles_m + 31) / 32 * 32 : tile_rows.most;
   return {lo, seg_row[lo] + mt * rows, min(rows, cnt - mt * rows), local / tiles_m};
 }
 
@@ -234,7 +253,8 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int n_tiles = (p.n + 127) / 128;
-  if (warp == 0) int8_stage_segments(p, TN, n_tiles, seg_row, seg_cnt, seg_end, lane);
+  constexpr Int8FixedRows<TN> kRows;
+  if (warp == 0) int8_stage_segments(p, kRows, n_tiles, seg_row, seg_cnt, seg_end, lane);
   ptx::tcgen05_fence_before_sync();
   __syncthreads();
   ptx::tcgen05_fence_after_sync();
@@ -251,7 +271,7 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
       bool ok = true;
       for (int tile = first; ok && tile < total; tile += step) {
         const Int8Tile t =
-            int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+            int8_find_tile<false>(tile, kRows, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
         const int wrow = t.expert * p.n + t.nt * 128;
         // Tokens come in one box of TN rows, or in boxes of 32 where half the rows are enough.
         const int boxes = (t.rows + 31) / 32;
@@ -312,7 +332,7 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
         ptx::tcgen05_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * Cfg::kAccCols;
         const Int8Tile t =
-            int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+            int8_find_tile<false>(tile, kRows, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
         const uint32_t idesc = ptx::make_idesc_i8(128, (t.rows + 15) / 16 * 16);
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&full_bar[stage], phase, abort_flag, p.error_bits, kDevErrMmaTimeout)) {
@@ -361,7 +381,7 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
     uint32_t local = 0;
     for (int tile = first; tile < total; tile += step, ++local) {
       const Int8Tile t =
-          int8_find_tile<false>(tile, TN, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
+          int8_find_tile<false>(tile, kRows, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
       const int n = t.nt * 128 + 32 * quarter + lane;
       const bool in = n < p.n;
       const int64_t chan = static_cast<int64_t>(t.expert) * p.n + n;

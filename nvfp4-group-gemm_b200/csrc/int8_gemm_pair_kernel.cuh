@@ -1,10 +1,10 @@
 // The int8 product on CTA pairs (cta_group::2), for segments of many rows.
 //
-// A cluster of two CTAs computes 256 weight rows x up to 256 tokens per tile: each CTA loads its
-// 128 weight rows and half of the tokens, so a token byte is brought to one SM only, and the
-// even CTA issues MMAs of M = 256 that read both CTAs' shared memory and leave each CTA's 128
-// rows in its own TMEM. All 512 TMEM columns hold two accumulators, so a tile's epilogue runs
-// under the next tile's MMAs.
+// A cluster of two CTAs computes 256 weight rows x up to pair_rows (at most 256) tokens per tile:
+// each CTA loads its 128 weight rows and half of the tokens, so a token byte is brought to one SM
+// only, and the even CTA issues MMAs of M = 256 that read both CTAs' shared memory and leave each
+// CTA's 128 rows in its own TMEM. All 512 TMEM columns hold two accumulators, so a tile's
+// epilogue runs under the next tile's MMAs.
 //
 // As in the single-CTA kernel, weight rows are TMEM lanes and tokens are columns. The MMA's N is
 // the tile's own token count (a multiple of 32), and an expert's tiles share its rows equally:
@@ -100,8 +100,9 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int n_tiles = (p.n + Cfg::kOutN - 1) / Cfg::kOutN;
+  const Int8PairRows tile_rows = {p.pair_rows, p.pair_inv};
   if (warp == 0)
-    int8_stage_segments(p, kInt8PairTokens, n_tiles, seg_row, seg_cnt, seg_end, lane);
+    int8_stage_segments(p, tile_rows, n_tiles, seg_row, seg_cnt, seg_end, lane);
   ptx::tcgen05_fence_before_sync();
   ptx::cluster_sync_all();
   ptx::tcgen05_fence_after_sync();
@@ -110,8 +111,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
   const int first = static_cast<int>(blockIdx.x >> 1);
   const int step = static_cast<int>(gridDim.x >> 1);
   auto find = [&](int tile) {
-    return int8_find_tile<true>(tile, kInt8PairTokens, n_tiles, p.num_experts, seg_row, seg_cnt,
-                                seg_end);
+    return int8_find_tile<true>(tile, tile_rows, n_tiles, p.num_experts, seg_row, seg_cnt, seg_end);
   };
   // N of a tile's MMAs: its tokens, 16 at a time from each CTA.
   auto mma_n = [](const Int8Tile& t) { return (t.rows + 31) / 32 * 32; };
@@ -126,11 +126,11 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
         const Int8Tile t = find(tile);
         const int half = mma_n(t) / 2;  // this CTA's tokens
         const int xrow = t.row + rank * half;
-        // In one box of 128 rows, or in boxes of 32 where half the rows are enough.
+        // In one box of pair_rows / 2 rows, or in boxes of 32 where half of them are enough.
         const int boxes = (half + 31) / 32;
-        const bool small = boxes <= 2;
+        const bool small = 128 * boxes <= p.pair_rows;
         const uint32_t bytes =
-            Cfg::kWBytes + (small ? 32 * boxes * kInt8StageK : Cfg::kXBytes);
+            Cfg::kWBytes + (small ? 32 * boxes : p.pair_rows / 2) * kInt8StageK;
         const int wrow = t.expert * p.n + t.nt * Cfg::kOutN + rank * Cfg::kWBox;
         for (int kt = 0; kt < p.ktiles; ++kt) {
           if (!wait_phase(&empty_bar[stage], phase ^ 1u, abort_flag, p.error_bits,

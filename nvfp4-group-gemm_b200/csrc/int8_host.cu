@@ -158,18 +158,48 @@ int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p,
 }
 
 template <bool GATED>
-int launch_int8_pair(const nvfp4_int8_product* g, const Int8GemmParams& p, int clusters,
+int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_rows, int clusters,
                      cudaStream_t s) {
   using Cfg = Int8PairConfig<GATED>;
   Int8Maps m;
-  if (!int8_maps(g, kInt8PairTokens / 2, Cfg::kWBox, &m))
+  p.pair_rows = tile_rows;
+  p.pair_inv = static_cast<uint32_t>(((int64_t{1} << 32) + tile_rows / 32 - 1) / (tile_rows / 32));
+  if (!int8_maps(g, tile_rows / 2, Cfg::kWBox, &m))
     return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
-  const int64_t tiles = int8_max_tiles(g, kInt8PairTokens, Cfg::kOutN);
+  const int64_t tiles = int8_max_tiles(g, tile_rows, Cfg::kOutN);
   if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
       launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED>, std::min<int64_t>(tiles, clusters) * 2,
                       2, kInt8PairThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
+}
+
+// Most tokens of a CTA pair's tile, for one segment: those whose waves of tiles end soonest. In
+// units of one token's MMAs over a stage, a stage takes the larger of its MMAs (tokens + 16) and
+// its loads (96 + tokens / 2), and a tile no less than its epilogue (8 per token and 1024), which
+// is not hidden behind the last tile. Fitted to 8192 x 4096 x 7168 (23.3 us a wave with 256
+// tokens, 15.1 with 160, 13.7 with 128, 12.3 with 96) and to short K. Against 256 tokens: 2537 x
+// 1806 x 7296 with 160 39.2 -> 30.2 us, 1536 x 1598 x 5253 with 160 22.3 -> 19.7, 700 x 4096 x
+// 7168 with 192 24.0 -> 19.6, 1453 x 4224 x 577 with 192 12.6 -> 11.0; 2048 x 4096 x 4096 keeps
+// 256 (26.8; 160 takes 27.6). Segments of several
+// experts keep 256, as their rows are not known here (by the average, 64 experts of 1024 +- 32
+// rows would lose 2 % and 64 of 128 +- 11 gain as much).
+template <bool GATED>
+int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
+  const int64_t n_tiles = (g->n + Int8PairConfig<GATED>::kOutN - 1) / Int8PairConfig<GATED>::kOutN;
+  int64_t best_cost = 0;
+  int best = 0;
+  for (int most = kInt8PairTokens; most >= 96; most -= 32) {
+    const int64_t row_tiles = (g->rows + most - 1) / most;
+    const int64_t equal = ((g->rows + row_tiles - 1) / row_tiles + 31) / 32 * 32;
+    const int64_t waves = (row_tiles * n_tiles + clusters - 1) / clusters;
+    const int64_t stage = std::max(equal + 16, 96 + equal / 2);
+    const int64_t cost = waves * std::max(ktiles * stage, 8 * equal + 1024) + 8 * equal;
+    if (best != 0 && 13 * cost >= 12 * best_cost) continue;  // a clear gain only
+    best_cost = cost;
+    best = static_cast<int>(equal);
+  }
+  return best;
 }
 
 // Kernel and tile of a product, from the rows that the segments are expected to hold. Times in us
@@ -211,7 +241,12 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
     return launch_int8_gemv_split<8, GATED>(g, p, active, num_sms, s);
   auto one_wave = [&](int tn) { return active * ((rows + tn - 1) / tn) * n_tiles <= num_sms; };
   const bool many = !one_wave(128);
-  if (many && rows > 80) return launch_int8_pair<GATED>(g, p, ds.pair_clusters, s);
+  if (many && rows > 80) {
+    const int tile_rows =
+        p.seg_offsets == nullptr ? int8_pair_rows<GATED>(g, p.ktiles, ds.pair_clusters)
+                                 : kInt8PairTokens;
+    return launch_int8_pair<GATED>(g, p, tile_rows, ds.pair_clusters, s);
+  }
   auto fits = [&](int tn) { return many ? 4 * tn >= 5 * rows : one_wave(tn); };
   if (fits(16)) return launch_int8<16, GATED>(g, p, num_sms, s);
   if (fits(32)) return launch_int8<32, GATED>(g, p, num_sms, s);

@@ -163,6 +163,21 @@ def test_product_of_every_kernel(pkg, m, n, k, dtype):
     assert pkg.check_int8_errors() == 0
 
 
+@pytest.mark.parametrize("m,n,k", [(993, 3090, 532), (861, 4811, 507), (858, 2859, 256),
+                                   (1291, 2418, 714), (1161, 2908, 960), (1001, 3934, 1398),
+                                   (97, 20000, 65), (600, 4200, 300), (1453, 4224, 577)])
+def test_product_on_cta_pairs_with_tiles_of_every_size(pkg, m, n, k):
+    """Rows and channels whose waves end soonest with tiles of 96, 128, ... 256 tokens, all of
+    them ragged; what surrounds the output is left as it was."""
+    a, b = _codes(m, k, 41), _codes(n, k, 42)
+    sa, sb = _scale(m, 43, 0.01), _scale(n, 44, 0.002)
+    out = torch.full((m + 2, n + 3), 7.0, dtype=torch.float16, device="cuda")
+    pkg.int8_gemm(a, sa, b, sb, out=out[:m, :n])
+    _check_product(out[:m, :n], a, sa, b, sb)
+    assert bool((out[m:] == 7).all()) and bool((out[:, n:] == 7).all())
+    assert pkg.check_int8_errors() == 0
+
+
 @pytest.mark.parametrize("n,k", [(2000, 8200), (300, 500), (1100, 4096), (500, 2047), (33, 1025)])
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8])
 def test_product_of_few_rows(pkg, m, n, k):
