@@ -27,33 +27,35 @@
 namespace nvfp4 {
 
 constexpr int kInt8PairTokens = 256;
-constexpr int kInt8PairEpiWarps = 8;
-constexpr int kInt8PairThreads = 64 + 32 * kInt8PairEpiWarps;
 
-template <bool GATED>
+// WARPS: of the epilogue, 8 or 16 (a tile's epilogue is a chain of latencies: with 8 warps 256
+// tokens took 3.9 us, gated 6.4, as long as the MMAs of K = 1300 and 2200; with 16 warps 3.6 and
+// 4.7, but long K ran 3 % slower beside them).
+template <bool GATED, int WARPS>
 struct Int8PairConfig {
   static constexpr int kOutN = GATED ? 128 : 256;   // channels of a tile
   static constexpr int kWBox = GATED ? 64 : 128;    // weight rows per load
   static constexpr int kWBytes = 128 * kInt8StageK;
   static constexpr int kXBytes = kInt8PairTokens / 2 * kInt8StageK;
   static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kStages = 6;
+  static constexpr int kThreads = 64 + 32 * WARPS;
+  static constexpr int kStages = GATED && WARPS > 8 ? 5 : 6;
   // Exchange of two warps: two buffers of 2 directions x 8 tokens x 32 channels.
   static constexpr int kPairBytes = 2 * 2 * 8 * 32 * 4;
-  static constexpr int kExchangeBytes = GATED ? kInt8PairEpiWarps / 2 * kPairBytes : 0;
+  static constexpr int kExchangeBytes = GATED ? WARPS / 2 * kPairBytes : 0;
   static constexpr int kSmemBytes =
       1024 + kStages * kStageBytes + kExchangeBytes + kInt8SegBytes + 512;
   static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory per CTA");
 };
 
-template <bool GATED>
-__global__ void __launch_bounds__(kInt8PairThreads, 1)
+template <bool GATED, int WARPS>
+__global__ void __launch_bounds__(64 + 32 * WARPS, 1)
     nvfp4_int8_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                                 const __grid_constant__ CUtensorMap map_a32,
                                 const __grid_constant__ CUtensorMap map_b,
                                 const __grid_constant__ CUtensorMap map_b2,
                                 const __grid_constant__ Int8GemmParams p) {
-  using Cfg = Int8PairConfig<GATED>;
+  using Cfg = Int8PairConfig<GATED, WARPS>;
   constexpr int kStages = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
   uint64_t* acce_bar = accf_bar + 2;
   uint64_t* drain_bar = acce_bar + 2;
   uint64_t* swap_bar = drain_bar + 1;  // one per two warps that exchange
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(swap_bar + 4);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(swap_bar + WARPS / 2);
   volatile uint32_t* abort_flag = tmem_holder + 1;
 
   const int warp = threadIdx.x >> 5;
@@ -83,9 +85,9 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(&accf_bar[a], 1);
-      ptx::mbar_init(&acce_bar[a], 2 * kInt8PairEpiWarps);
+      ptx::mbar_init(&acce_bar[a], 2 * WARPS);
     }
-    for (int i = 0; i < 4; ++i) ptx::mbar_init(&swap_bar[i], 2);
+    for (int i = 0; i < WARPS / 2; ++i) ptx::mbar_init(&swap_bar[i], 2);
     ptx::mbar_init(drain_bar, 1);
     *abort_flag = 0u;
     ptx::fence_mbarrier_init();
@@ -223,10 +225,12 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
-    const int odd = (warp - kEpilogueWarp0) / 4;  // takes the odd chunks of 16 tokens
+    constexpr int kStep = 4 * WARPS;  // tokens between a warp's chunks of 16
+    constexpr int kChunks = kInt8PairTokens / kStep;
+    const int turn = (warp - kEpilogueWarp0) / 4;  // its first chunk
     const bool up = GATED && quarter >= 2;
     const int group = GATED ? quarter & 1 : quarter;  // 32 channels of the CTA's
-    float* swap = exchange + (2 * odd + group) * (Cfg::kPairBytes / 4) + lane;
+    float* swap = exchange + (2 * turn + group) * (Cfg::kPairBytes / 4) + lane;
     uint32_t full_parity = 0;
     uint32_t local = 0;
     uint32_t swaps = 0;
@@ -238,11 +242,11 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
       const int64_t chan = static_cast<int64_t>(t.expert) * p.n + n;
       const float bs = in ? __ldg((up ? p.b2_scale : p.b_scale) + chan) : 0.0f;
       const float bias = !GATED && in && p.bias != nullptr ? __ldg(p.bias + n) : 0.0f;
-      // Token scales: lane l of as[j] holds those of tokens 64 j + 32 (l / 16) + 16 odd + l % 16.
-      float as[4];
+      // Token scales: lane l of as[j] holds that of token l % 16 of the warp's chunk 2 j + l / 16.
+      float as[kChunks / 2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = 64 * j + 32 * (lane >> 4) + 16 * odd + (lane & 15);
+      for (int j = 0; j < kChunks / 2; ++j) {
+        const int tok = kStep * (2 * j + (lane >> 4)) + 16 * turn + (lane & 15);
         as[j] = tok < t.rows ? __ldg(p.a_scale + t.row + tok) : 0.0f;
       }
       const int acc = static_cast<int>(local & 1u);
@@ -252,13 +256,13 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
       full_parity ^= 1u << acc;
       ptx::tcgen05_fence_after_sync();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) +
-                             acc * kInt8PairTokens + 16 * odd;
+                             acc * kInt8PairTokens + 16 * turn;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tok = 32 * j + 16 * odd;
+      for (int j = 0; j < kChunks; ++j) {
+        const int tok = kStep * j + 16 * turn;
         if (tok >= t.rows) break;  // uniform over the warp (and the two that exchange)
         uint32_t v[16];
-        ptx::tmem_ld_32x32b_x16(t_acc + 32 * j, v);
+        ptx::tmem_ld_32x32b_x16(t_acc + kStep * j, v);
         ptx::tmem_ld_wait();
         ptx::reg_fence(v);
         float y[16];
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
 #pragma unroll
           for (int i = 0; i < 8; ++i) to[32 * i] = up ? y[i] : y[8 + i];
           __syncwarp();
-          uint64_t* bar = &swap_bar[2 * odd + group];
+          uint64_t* bar = &swap_bar[2 * turn + group];
           if (lane == 0) ptx::mbar_arrive(bar);
           if (!warp_wait_phase(bar, swaps & 1u, abort_flag, p.error_bits, kDevErrEpilogueTimeout,
                                lane)) {

@@ -35,16 +35,21 @@ cudaError_t allow_smem() {
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Int8Config<TN, GATED>::kSmemBytes);
 }
+template <bool GATED, int WARPS>
+cudaError_t allow_smem_pair() {
+  return cudaFuncSetAttribute(nvfp4_int8_gemm_pair_kernel<GATED, WARPS>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Int8PairConfig<GATED, WARPS>::kSmemBytes);
+}
+
 template <bool GATED>
 cudaError_t allow_smem_all() {
   cudaError_t e = allow_smem<16, GATED>();
   if (e == cudaSuccess) e = allow_smem<32, GATED>();
   if (e == cudaSuccess) e = allow_smem<64, GATED>();
   if (e == cudaSuccess) e = allow_smem<128, GATED>();
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(nvfp4_int8_gemm_pair_kernel<GATED>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Int8PairConfig<GATED>::kSmemBytes);
+  if (e == cudaSuccess) e = allow_smem_pair<GATED, 8>();
+  if (e == cudaSuccess) e = allow_smem_pair<GATED, 16>();
   return e;
 }
 
@@ -157,10 +162,10 @@ int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p,
   return launch_int8_gemv<TB, R, 1, GATED>(g, p, num_sms, s);
 }
 
-template <bool GATED>
+template <bool GATED, int WARPS>
 int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_rows, int clusters,
                      cudaStream_t s) {
-  using Cfg = Int8PairConfig<GATED>;
+  using Cfg = Int8PairConfig<GATED, WARPS>;
   Int8Maps m;
   p.pair_rows = tile_rows;
   p.pair_inv = static_cast<uint32_t>(((int64_t{1} << 32) + tile_rows / 32 - 1) / (tile_rows / 32));
@@ -169,8 +174,8 @@ int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_row
   const int64_t tiles = int8_max_tiles(g, tile_rows, Cfg::kOutN);
   if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
-      launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED>, std::min<int64_t>(tiles, clusters) * 2,
-                      2, kInt8PairThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
+      launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED, WARPS>,
+                      std::min<int64_t>(tiles, clusters) * 2, 2, Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
@@ -186,7 +191,8 @@ int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_row
 // rows would lose 2 % and 64 of 128 +- 11 gain as much).
 template <bool GATED>
 int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
-  const int64_t n_tiles = (g->n + Int8PairConfig<GATED>::kOutN - 1) / Int8PairConfig<GATED>::kOutN;
+  constexpr int kOutN = Int8PairConfig<GATED, 8>::kOutN;
+  const int64_t n_tiles = (g->n + kOutN - 1) / kOutN;
   int64_t best_cost = 0;
   int best = 0;
   for (int most = kInt8PairTokens; most >= 96; most -= 32) {
@@ -219,7 +225,10 @@ int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
 // chosen to hold them with a quarter to spare (64 experts of 64 +- 8 rows, N 4096, K 1536:
 // 70.5 with 128 tokens, 75.6 with 64); above 80 rows the MMAs decide and CTA pairs are faster
 // (128 rows: 81 against 97 with 128-token tiles, gated N 1536, K 4096 155 against 159;
-// 64 rows: 141 against 137).
+// 64 rows: 141 against 137). Pairs take 16 epilogue warps up to the K at which a tile's MMAs hide
+// what 8 of them do (16 experts of 2048 rows, 8 and 16 warps: gated N 1024, K 1024 101 and 77 us,
+// K 2048 115 and 104, K 3000 146 and 149; plain N 2048, K 512 62.5 and 56, K 1024 69.6 and 65.9,
+// K 2048 100.7 and 102.8).
 template <bool GATED>
 int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const DeviceState& ds,
                 cudaStream_t s) {
@@ -245,7 +254,9 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
     const int tile_rows =
         p.seg_offsets == nullptr ? int8_pair_rows<GATED>(g, p.ktiles, ds.pair_clusters)
                                  : kInt8PairTokens;
-    return launch_int8_pair<GATED>(g, p, tile_rows, ds.pair_clusters, s);
+    return p.ktiles <= (GATED ? 18 : 8)
+               ? launch_int8_pair<GATED, 16>(g, p, tile_rows, ds.pair_clusters, s)
+               : launch_int8_pair<GATED, 8>(g, p, tile_rows, ds.pair_clusters, s);
   }
   auto fits = [&](int tn) { return many ? 4 * tn >= 5 * rows : one_wave(tn); };
   if (fits(16)) return launch_int8<16, GATED>(g, p, num_sms, s);

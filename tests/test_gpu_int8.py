@@ -265,6 +265,18 @@ def _segments_case(pkg, offs, cnts, rows, n, k, gated, dtype, expected, seed=0):
     return out
 
 
+@pytest.mark.parametrize("k", [700, 1025, 2304, 2305])
+@pytest.mark.parametrize("gated", [False, True])
+def test_segments_on_cta_pairs_with_short_and_long_sums(pkg, gated, k):
+    """CTA pairs with 16 epilogue warps (short K) and with 8: counts that leave warps without
+    tokens in a tile, and an expert without rows."""
+    cnts = [17, 256, 0, 289, 513, 33, 241]
+    offs = np.concatenate([[1], 1 + np.cumsum(cnts)[:-1] + np.arange(1, 7)]).tolist()
+    _segments_case(pkg, offs, cnts, offs[-1] + cnts[-1] + 3, 1701, k, gated, torch.bfloat16,
+                   sum(cnts), seed=k)
+    assert pkg.check_int8_errors() == 0
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("offs,cnts,expected", [
     ([0], [1], 1),
