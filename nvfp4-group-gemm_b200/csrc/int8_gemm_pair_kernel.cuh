@@ -1,4 +1,4 @@
-// The int8 product on CTA pairs (cta_group::2), for segments of many rows.
+// The int8 product on CTA pairs (cta_group::2), for segments of many rows (gated: and long K).
 //
 // A cluster of two CTAs computes 256 weight rows x up to pair_rows (at most 256) tokens per tile:
 // each CTA loads its 128 weight rows and half of the tokens, so a token byte is brought to one SM

@@ -225,10 +225,12 @@ int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
 // chosen to hold them with a quarter to spare (64 experts of 64 +- 8 rows, N 4096, K 1536:
 // 70.5 with 128 tokens, 75.6 with 64); above 80 rows the MMAs decide and CTA pairs are faster
 // (128 rows: 81 against 97 with 128-token tiles, gated N 1536, K 4096 155 against 159;
-// 64 rows: 141 against 137). Pairs take 16 epilogue warps up to the K at which a tile's MMAs hide
-// what 8 of them do (16 experts of 2048 rows, 8 and 16 warps: gated N 1024, K 1024 101 and 77 us,
-// K 2048 115 and 104, K 3000 146 and 149; plain N 2048, K 512 62.5 and 56, K 1024 69.6 and 65.9,
-// K 2048 100.7 and 102.8).
+// 64 rows: 141 against 137). Gated sums of short K stay on single CTAs, whose epilogue has both
+// sums of a channel in one lane (16 experts of 2048 rows, N 1024, single and pair: K 512 57 and
+// 75 us, K 1024 65 and 78, K 1536 88 and 87, K 2048 110 and 102). Pairs take 16 epilogue warps up
+// to the K at which a tile's MMAs hide what 8 of them do (8 and 16 warps: these experts, K 1536
+// 104 and 88, K 2048 115 and 104, K 3000 146 and 149; plain N 2048, K 512 62.5 and 56, K 1024 69.6
+// and 65.9, K 2048 100.7 and 102.8).
 template <bool GATED>
 int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const DeviceState& ds,
                 cudaStream_t s) {
@@ -250,7 +252,7 @@ int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const Devi
     return launch_int8_gemv_split<8, GATED>(g, p, active, num_sms, s);
   auto one_wave = [&](int tn) { return active * ((rows + tn - 1) / tn) * n_tiles <= num_sms; };
   const bool many = !one_wave(128);
-  if (many && rows > 80) {
+  if (many && rows > 80 && (!GATED || p.ktiles > 10)) {
     const int tile_rows =
         p.seg_offsets == nullptr ? int8_pair_rows<GATED>(g, p.ktiles, ds.pair_clusters)
                                  : kInt8PairTokens;
