@@ -36,7 +36,8 @@ extern "C" {
 /* 3: int8 products (nvfp4_int8_gemm, nvfp4_quantize_int8, nvfp4_moe_dispatch_int8), token sort
  * with gradients (nvfp4_moe_dispatch_tokens, nvfp4_moe_combine_tokens and its backward),
  * NVFP4_DTYPE_FP32. */
-#define NVFP4_ABI_VERSION 3
+/* 4: nvfp4_int8_plan. */
+#define NVFP4_ABI_VERSION 4
 
 typedef enum nvfp4_status {
   NVFP4_OK = 0,
@@ -385,6 +386,23 @@ typedef struct nvfp4_int8_product {
 } nvfp4_int8_product;
 
 NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* product, void* stream);
+
+/*
+ * What nvfp4_int8_gemm launches for a product on a GPU of num_sms SMs that runs cta_pairs
+ * clusters of two CTAs at once. Decided on the host from the record alone: nothing is launched
+ * and no GPU is needed. All zeros for a product of no rows.
+ */
+#define NVFP4_INT8_BYTES 1 /* byte products: `tokens` rows per pass, `warps` share K */
+#define NVFP4_INT8_TILES 2 /* single CTAs: tiles of `tokens` rows, `warps` in the epilogue */
+#define NVFP4_INT8_PAIRS 3 /* CTA pairs: tiles of up to `tokens` rows, `warps` in the epilogue */
+typedef struct nvfp4_int8_launch {
+  int32_t kernel;
+  int32_t tokens;
+  int32_t warps;
+} nvfp4_int8_launch;
+
+NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* product, int num_sms, int cta_pairs,
+                              nvfp4_int8_launch* launch);
 
 /*
  * Synchronise `stream`, then read and clear the current device's error word of the int8

@@ -86,10 +86,11 @@ EXPORTED_SYMBOLS = (
     "nvfp4_quantize_int8",
     "nvfp4_moe_dispatch_int8",
     "nvfp4_int8_gemm",
+    "nvfp4_int8_plan",
     "nvfp4_int8_check",
 )
 
-ABI_VERSION = 3   # NVFP4_ABI_VERSION
+ABI_VERSION = 4   # NVFP4_ABI_VERSION
 EP_MAX_RANKS = 8  # NVFP4_EP_MAX_RANKS
 MAX_REPLICAS = 7  # replicas nvfp4_grouped_gemm_replicated accepts
 EP_ERR_CAPACITY = 1 << 0  # an expert segment did not fit the owner's receive slab
@@ -197,7 +198,19 @@ class Int8Product(ctypes.Structure):
     ]
 
 
-# The same record packed in one step (its fields in order, 0 for NULL): the bytes are passed as
+class Int8Launch(ctypes.Structure):
+    """Mirror of ``nvfp4_int8_launch``."""
+
+    _fields_ = [("kernel", ctypes.c_int32), ("tokens", ctypes.c_int32), ("warps", ctypes.c_int32)]
+
+
+# Kernels of an int8 product (NVFP4_INT8_*).
+INT8_BYTES = 1
+INT8_TILES = 2
+INT8_PAIRS = 3
+
+
+# Int8Product packed in one step (its fields in order, 0 for NULL): the bytes are passed as
 # they are, at a third of the time that filling the ctypes structure takes.
 pack_int8_product = struct.Struct("<10Q5q4i").pack
 assert len(pack_int8_product(*[0] * 19)) == ctypes.sizeof(Int8Product)
@@ -336,6 +349,8 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.nvfp4_moe_dispatch_int8.restype = i32
         lib.nvfp4_int8_gemm.argtypes = [vp, vp]
         lib.nvfp4_int8_gemm.restype = i32
+        lib.nvfp4_int8_plan.argtypes = [vp, i32, i32, ctypes.POINTER(Int8Launch)]
+        lib.nvfp4_int8_plan.restype = i32
         lib.nvfp4_int8_check.argtypes = [vp, ctypes.POINTER(ctypes.c_uint)]
         lib.nvfp4_int8_check.restype = i32
         if path is None:

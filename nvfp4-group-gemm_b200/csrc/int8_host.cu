@@ -80,6 +80,14 @@ int int8_device(Int8Device** out, DeviceState** state) {
   return NVFP4_OK;
 }
 
+int int8_ktiles(const nvfp4_int8_product* g) { return (g->k + kInt8StageK - 1) / kInt8StageK; }
+
+// What a product launches: one of NVFP4_INT8_*, the most tokens that a tile (or a pass over the
+// weights) takes, and the warps that share K or drain the accumulators.
+struct Int8Plan {
+  int kernel, tokens, warps;
+};
+
 // int8 rows [rows, k], `ld` bytes apart, in boxes of 128 bytes x box_rows, 128-byte swizzle,
 // zero fill past the last column and row.
 bool int8_map(CUtensorMap* m, const void* addr, int64_t rows, int k, int64_t ld, int box_rows) {
@@ -128,6 +136,10 @@ int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sm
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
+// Channels (R) of a group of warps: two, four where more tokens' codes have to be loaded for them
+// (four tokens, N 2048, K 2048: 4.0 us against 4.6).
+constexpr int int8_gemv_channels(int tokens, bool gated) { return tokens <= 2 || gated ? 2 : 4; }
+
 template <int TB, int R, int KS, bool GATED>
 int launch_int8_gemv(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sms,
                      cudaStream_t s) {
@@ -147,18 +159,13 @@ int launch_int8_gemv(const nvfp4_int8_product* g, const Int8GemmParams& p, int n
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
-// Warps of a group (KS): as many as keep the warps within one wave (32 per SM) and leave each
-// two loads of 512 bytes of K. Channels of a group (R): two, four where more tokens' codes have
-// to be loaded for them (four tokens, N 2048, K 2048: 4.0 us against 4.6).
 template <int TB, bool GATED>
-int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p, int64_t active,
+int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p, int warps,
                            int num_sms, cudaStream_t s) {
-  constexpr int R = TB <= 2 || GATED ? 2 : 4;
-  const int64_t groups = (static_cast<int64_t>(g->n) + R - 1) / R * active;
-  auto fits = [&](int ks) { return groups * ks <= num_sms * 32 && g->k >= 1024 * ks; };
-  if (fits(8)) return launch_int8_gemv<TB, R, 8, GATED>(g, p, num_sms, s);
-  if (fits(4)) return launch_int8_gemv<TB, R, 4, GATED>(g, p, num_sms, s);
-  if (fits(2)) return launch_int8_gemv<TB, R, 2, GATED>(g, p, num_sms, s);
+  constexpr int R = int8_gemv_channels(TB, GATED);
+  if (warps == 8) return launch_int8_gemv<TB, R, 8, GATED>(g, p, num_sms, s);
+  if (warps == 4) return launch_int8_gemv<TB, R, 4, GATED>(g, p, num_sms, s);
+  if (warps == 2) return launch_int8_gemv<TB, R, 2, GATED>(g, p, num_sms, s);
   return launch_int8_gemv<TB, R, 1, GATED>(g, p, num_sms, s);
 }
 
@@ -189,9 +196,8 @@ int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_row
 // 256 (26.8; 160 takes 27.6). Segments of several
 // experts keep 256, as their rows are not known here (by the average, 64 experts of 1024 +- 32
 // rows would lose 2 % and 64 of 128 +- 11 gain as much).
-template <bool GATED>
-int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
-  constexpr int kOutN = Int8PairConfig<GATED, 8>::kOutN;
+int int8_pair_rows(const nvfp4_int8_product* g, bool gated, int ktiles, int clusters) {
+  const int kOutN = gated ? Int8PairConfig<true, 8>::kOutN : Int8PairConfig<false, 8>::kOutN;
   const int64_t n_tiles = (g->n + kOutN - 1) / kOutN;
   int64_t best_cost = 0;
   int best = 0;
@@ -231,40 +237,59 @@ int int8_pair_rows(const nvfp4_int8_product* g, int ktiles, int clusters) {
 // to the K at which a tile's MMAs hide what 8 of them do (8 and 16 warps: these experts, K 1536
 // 104 and 88, K 2048 115 and 104, K 3000 146 and 149; plain N 2048, K 512 62.5 and 56, K 1024 69.6
 // and 65.9, K 2048 100.7 and 102.8).
-template <bool GATED>
-int choose_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, const DeviceState& ds,
-                cudaStream_t s) {
-  const int num_sms = ds.num_sms;
+Int8Plan plan_int8(const nvfp4_int8_product* g, int num_sms, int clusters) {
+  const bool gated = g->b2 != nullptr;
+  const int ktiles = int8_ktiles(g);
   const int64_t expected = g->expected_rows > 0 ? std::min(g->expected_rows, g->rows) : g->rows;
   const int64_t active = std::min<int64_t>(g->num_experts, expected);  // experts with rows
   const int64_t rows = (expected + active - 1) / active;
   const int64_t n_tiles = (g->n + 127) / 128;
   const int64_t tiles = active * n_tiles;
+  // Warps of a group (KS): as many as keep the warps within one wave (32 per SM) and leave each
+  // two loads of 512 bytes of K.
+  auto bytes = [&](int tokens) {
+    const int r = int8_gemv_channels(tokens, gated);
+    const int64_t groups = (static_cast<int64_t>(g->n) + r - 1) / r * active;
+    int warps = 8;
+    while (warps > 1 && (groups * warps > num_sms * 32 || g->k < 1024 * warps)) warps /= 2;
+    return Int8Plan{NVFP4_INT8_BYTES, tokens, warps};
+  };
   // Experts' counts vary: twice the average, unless each is expected to have one row.
   const int64_t at_once = g->num_experts > 1 && rows > 1 ? 2 * rows : rows;
-  if (at_once == 1 && tiles < num_sms)
-    return launch_int8_gemv_split<1, GATED>(g, p, active, num_sms, s);
-  if (at_once == 2 && tiles < num_sms)
-    return launch_int8_gemv_split<2, GATED>(g, p, active, num_sms, s);
-  if (at_once <= 4 && (GATED ? 4 : 2) * tiles < num_sms && g->k >= 1024)
-    return launch_int8_gemv_split<4, GATED>(g, p, active, num_sms, s);
-  if (at_once <= 8 && 9 * tiles < num_sms && g->k >= 2048)
-    return launch_int8_gemv_split<8, GATED>(g, p, active, num_sms, s);
+  if (at_once == 1 && tiles < num_sms) return bytes(1);
+  if (at_once == 2 && tiles < num_sms) return bytes(2);
+  if (at_once <= 4 && (gated ? 4 : 2) * tiles < num_sms && g->k >= 1024) return bytes(4);
+  if (at_once <= 8 && 9 * tiles < num_sms && g->k >= 2048) return bytes(8);
   auto one_wave = [&](int tn) { return active * ((rows + tn - 1) / tn) * n_tiles <= num_sms; };
   const bool many = !one_wave(128);
-  if (many && rows > 80 && (!GATED || p.ktiles > 10)) {
-    const int tile_rows =
-        p.seg_offsets == nullptr ? int8_pair_rows<GATED>(g, p.ktiles, ds.pair_clusters)
-                                 : kInt8PairTokens;
-    return p.ktiles <= (GATED ? 18 : 8)
-               ? launch_int8_pair<GATED, 16>(g, p, tile_rows, ds.pair_clusters, s)
-               : launch_int8_pair<GATED, 8>(g, p, tile_rows, ds.pair_clusters, s);
+  if (many && rows > 80 && (!gated || ktiles > 10)) {
+    const int tile_rows = g->seg_offsets == nullptr ? int8_pair_rows(g, gated, ktiles, clusters)
+                                                    : kInt8PairTokens;
+    return {NVFP4_INT8_PAIRS, tile_rows, ktiles <= (gated ? 18 : 8) ? 16 : 8};
   }
   auto fits = [&](int tn) { return many ? 4 * tn >= 5 * rows : one_wave(tn); };
-  if (fits(16)) return launch_int8<16, GATED>(g, p, num_sms, s);
-  if (fits(32)) return launch_int8<32, GATED>(g, p, num_sms, s);
-  if (fits(64)) return launch_int8<64, GATED>(g, p, num_sms, s);
-  return launch_int8<128, GATED>(g, p, num_sms, s);
+  int tn = 16;
+  while (tn < 128 && !fits(tn)) tn *= 2;
+  return {NVFP4_INT8_TILES, tn, tn >= 64 ? 8 : 4};
+}
+
+template <bool GATED>
+int launch_plan_int8(const Int8Plan& plan, const nvfp4_int8_product* g, const Int8GemmParams& p,
+                     const DeviceState& ds, cudaStream_t s) {
+  const int sms = ds.num_sms;
+  const int tokens = plan.tokens;
+  if (plan.kernel == NVFP4_INT8_BYTES)
+    return tokens == 1   ? launch_int8_gemv_split<1, GATED>(g, p, plan.warps, sms, s)
+           : tokens == 2 ? launch_int8_gemv_split<2, GATED>(g, p, plan.warps, sms, s)
+           : tokens == 4 ? launch_int8_gemv_split<4, GATED>(g, p, plan.warps, sms, s)
+                         : launch_int8_gemv_split<8, GATED>(g, p, plan.warps, sms, s);
+  if (plan.kernel == NVFP4_INT8_PAIRS)
+    return plan.warps == 16 ? launch_int8_pair<GATED, 16>(g, p, tokens, ds.pair_clusters, s)
+                            : launch_int8_pair<GATED, 8>(g, p, tokens, ds.pair_clusters, s);
+  return tokens == 16   ? launch_int8<16, GATED>(g, p, sms, s)
+         : tokens == 32 ? launch_int8<32, GATED>(g, p, sms, s)
+         : tokens == 64 ? launch_int8<64, GATED>(g, p, sms, s)
+                        : launch_int8<128, GATED>(g, p, sms, s);
 }
 
 template <typename T, int G, int V>
@@ -338,34 +363,8 @@ int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dt
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 quantiser launch");
 }
 
-}  // namespace
-}  // namespace nvfp4
-
-using namespace nvfp4;
-
-extern "C" {
-
-NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
-                                  const int32_t* row_list, int64_t listed, void* codes,
-                                  int64_t codes_ld, float* scales, void* stream) {
-  g_last_error.clear();
-  return quantize_int8_impl(x, rows, cols, ld, dtype, row_list, row_list != nullptr ? listed : 0,
-                            nullptr, 1, rows, codes, codes_ld, scales, stream);
-}
-
-NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
-                                      const int32_t* dest, int topk, int64_t rows, void* codes,
-                                      int64_t codes_ld, float* scales, void* stream) {
-  g_last_error.clear();
-  if (topk <= 0 || static_cast<int64_t>(tokens) * topk > (int64_t{1} << 30))
-    return fail(NVFP4_ERR_BAD_SHAPE, "tokens=%d topk=%d", tokens, topk);
-  if (tokens > 0 && dest == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "dest is NULL");
-  return quantize_int8_impl(x, tokens, cols, ld, dtype, nullptr, 0, dest, topk, rows, codes, codes_ld,
-                            scales, stream);
-}
-
-NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
-  g_last_error.clear();
+// Checks of a product's record that need no GPU.
+int check_product(const nvfp4_int8_product* g) {
   if (g == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "product is NULL");
   if (g->num_experts <= 0 || g->num_experts > kInt8MaxExperts)
     return fail(NVFP4_ERR_INVALID_ARGUMENT, "num_experts=%d must be in [1, %d]", g->num_experts,
@@ -397,6 +396,56 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
       g->ldb % 16 != 0)
     return fail(NVFP4_ERR_MISALIGNED,
                 "operands must be 16-byte aligned, lda and ldb multiples of 16 bytes");
+  return NVFP4_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" {
+
+NVFP4_API int nvfp4_quantize_int8(const void* x, int64_t rows, int cols, int64_t ld, int dtype,
+                                  const int32_t* row_list, int64_t listed, void* codes,
+                                  int64_t codes_ld, float* scales, void* stream) {
+  g_last_error.clear();
+  return quantize_int8_impl(x, rows, cols, ld, dtype, row_list, row_list != nullptr ? listed : 0,
+                            nullptr, 1, rows, codes, codes_ld, scales, stream);
+}
+
+NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64_t ld, int dtype,
+                                      const int32_t* dest, int topk, int64_t rows, void* codes,
+                                      int64_t codes_ld, float* scales, void* stream) {
+  g_last_error.clear();
+  if (topk <= 0 || static_cast<int64_t>(tokens) * topk > (int64_t{1} << 30))
+    return fail(NVFP4_ERR_BAD_SHAPE, "tokens=%d topk=%d", tokens, topk);
+  if (tokens > 0 && dest == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "dest is NULL");
+  return quantize_int8_impl(x, tokens, cols, ld, dtype, nullptr, 0, dest, topk, rows, codes, codes_ld,
+                            scales, stream);
+}
+
+NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* g, int num_sms, int cta_pairs,
+                              nvfp4_int8_launch* launch) {
+  g_last_error.clear();
+  const int bad = check_product(g);
+  if (bad != NVFP4_OK) return bad;
+  if (launch == nullptr) return fail(NVFP4_ERR_NULL_POINTER, "launch is NULL");
+  if (num_sms <= 0 || cta_pairs <= 0)
+    return fail(NVFP4_ERR_INVALID_ARGUMENT, "num_sms=%d cta_pairs=%d", num_sms, cta_pairs);
+  *launch = {};
+  if (g->rows == 0) return NVFP4_OK;
+  const Int8Plan plan = plan_int8(g, num_sms, cta_pairs);
+  launch->kernel = plan.kernel;
+  launch->tokens = plan.tokens;
+  launch->warps = plan.warps;
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
+  g_last_error.clear();
+  const int bad = check_product(g);
+  if (bad != NVFP4_OK || g->rows == 0) return bad;
   Int8Device* d = nullptr;
   DeviceState* ds = nullptr;
   const int st = int8_device(&d, &ds);
@@ -413,13 +462,15 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
   p.error_bits = d->error_bits;
   p.rows = static_cast<int32_t>(g->rows);
   p.n = g->n;
-  p.ktiles = (g->k + kInt8StageK - 1) / kInt8StageK;
+  p.ktiles = int8_ktiles(g);
   p.num_experts = g->num_experts;
   p.out_dtype = g->out_dtype == NVFP4_DTYPE_BF16   ? kInt8OutBf16
                 : g->out_dtype == NVFP4_DTYPE_FP16 ? kInt8OutFp16
                                                    : kInt8OutFp32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return gated ? choose_int8<true>(g, p, *ds, s) : choose_int8<false>(g, p, *ds, s);
+  const Int8Plan plan = plan_int8(g, ds->num_sms, ds->pair_clusters);
+  return g->b2 != nullptr ? launch_plan_int8<true>(plan, g, p, *ds, s)
+                          : launch_plan_int8<false>(plan, g, p, *ds, s);
 }
 
 NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits) {

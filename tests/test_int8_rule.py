@@ -1,0 +1,52 @@
+"""The rule that chooses an int8 product's kernel and tile, as the host reports it (CPU only)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+import int8_cases as C
+
+
+@pytest.mark.parametrize("counts,n,k,warps", C.GATED_PAIRS)
+def test_gated_pairs(pkg, counts, n, k, warps):
+    _, rows = C.offsets(counts)
+    assert C.plan(pkg, rows, n, k, len(counts), True, sum(counts), True) == (C.PAIRS, 256, warps)
+
+
+@pytest.mark.parametrize("gated,k,warps", C.EIGHT_ROWS)
+def test_byte_products_of_eight_rows(pkg, gated, k, warps):
+    _, rows = C.offsets(C.EIGHT_COUNTS)
+    got = C.plan(pkg, rows, C.EIGHT_N, k, len(C.EIGHT_COUNTS), gated, C.EIGHT_EXPECTED, True)
+    assert got == (C.BYTES, 8, warps)
+
+
+@pytest.mark.parametrize("rows,k,warps", C.ONE_EXPERT)
+def test_byte_products_of_one_expert(pkg, rows, k, warps):
+    assert C.plan(pkg, rows, C.ONE_EXPERT_N, k, 1, True, rows, True) == (C.BYTES, rows, warps)
+
+
+def test_short_gated_sums_stay_on_single_ctas(pkg):
+    _, rows = C.offsets(C.RAGGED)
+    for k, kernel in ((1280, C.TILES), (1281, C.PAIRS)):
+        assert C.plan(pkg, rows, 1701, k, len(C.RAGGED), True, sum(C.RAGGED), True)[0] == kernel
+        assert C.plan(pkg, rows, 3402, k, len(C.RAGGED), False, sum(C.RAGGED), True)[0] == C.PAIRS
+
+
+def test_dense_products(pkg):
+    assert C.plan(pkg, 1, 4096, 7168) == (C.BYTES, 1, 2)
+    assert C.plan(pkg, 83, 4099, 2011) == (C.TILES, 32, 4)
+    assert C.plan(pkg, 8192, 4096, 7168) == (C.PAIRS, 256, 8)
+    assert C.plan(pkg, 8192, 2048, 512)[::2] == (C.PAIRS, 16)
+    assert C.plan(pkg, 2537, 1806, 7296)[:2] == (C.PAIRS, 160)
+
+
+def test_of_no_rows_and_refusals(pkg):
+    assert C.plan(pkg, 0, 64, 64) == (0, 0, 0)
+    lib, N = pkg.load_library(), pkg._native
+    out = N.Int8Launch()
+    assert lib.nvfp4_int8_plan(None, 148, 74, ctypes.byref(out)) == 4
+    with pytest.raises(pkg.Nvfp4Error):
+        C.plan(pkg, 4, 64, 131072)
+    with pytest.raises(pkg.Nvfp4Error):
+        C.plan(pkg, 4, 64, 64, sms=0)
