@@ -399,6 +399,7 @@ typedef struct nvfp4_int8_launch {
   int32_t kernel;
   int32_t tokens;
   int32_t warps;
+  int32_t rows; /* of the first tile (pass) of a segment that holds all rows */
 } nvfp4_int8_launch;
 
 NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* product, int num_sms, int cta_pairs,

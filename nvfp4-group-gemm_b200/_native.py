@@ -201,7 +201,8 @@ class Int8Product(ctypes.Structure):
 class Int8Launch(ctypes.Structure):
     """Mirror of ``nvfp4_int8_launch``."""
 
-    _fields_ = [("kernel", ctypes.c_int32), ("tokens", ctypes.c_int32), ("warps", ctypes.c_int32)]
+    _fields_ = [("kernel", ctypes.c_int32), ("tokens", ctypes.c_int32), ("warps", ctypes.c_int32),
+                ("rows", ctypes.c_int32)]
 
 
 # Kernels of an int8 product (NVFP4_INT8_*).

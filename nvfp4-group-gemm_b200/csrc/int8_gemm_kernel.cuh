@@ -101,15 +101,24 @@ __device__ __forceinline__ float int8_silu_mul(float g, float u) {
 template <int ROWS>
 struct Int8FixedRows {
   static constexpr int most = ROWS;
-  __device__ __forceinline__ int tiles(int count) const { return (count + ROWS - 1) / ROWS; }
+  __host__ __device__ __forceinline__ int tiles(int count) const {
+    return (count + ROWS - 1) / ROWS;
+  }
 };
 struct Int8PairRows {
   int most;
   uint32_t inv;
-  __device__ __forceinline__ int tiles(int count) const {
-    return static_cast<int>(__umulhi((static_cast<uint32_t>(count) + most - 1) / 32, inv));
+  __host__ __device__ __forceinline__ int tiles(int count) const {
+    const uint32_t v = (static_cast<uint32_t>(count) + most - 1) / 32;
+    return static_cast<int>(static_cast<uint64_t>(v) * inv >> 32);
   }
 };
+
+// Rows of each of `tiles` equal tiles of `count` >= 1 rows (a multiple of 32), the last one aside;
+// no sum passes 2^31, whatever the count.
+__host__ __device__ __forceinline__ int int8_equal_rows(int count, int tiles) {
+  return ((count - 1) / tiles + 32) / 32 * 32;
+}
 
 // Segments of the launch in shared memory: first row, rows, and the end of each expert's tile
 // range. Warp-wide; a segment outside the slab is skipped and reported, and so is one with which
@@ -183,7 +192,7 @@ __device__ __forceinline__ Int8Tile int8_find_tile(int tile, Rows tile_rows, int
   const int tiles_m = tile_rows.tiles(cnt);
   const int local = tile - (seg_end[lo] - tiles_m * n_tiles);
   const int mt = local % tiles_m;
-  const int rows = BALANCED ? ((cnt + tiles_m - 1) / tiles_m + 31) / 32 * 32 : tile_rows.most;
+  const int rows = BALANCED ? int8_equal_rows(cnt, tiles_m) : tile_rows.most;
   return {lo, seg_row[lo] + mt * rows, min(rows, cnt - mt * rows), local / tiles_m};
 }
 

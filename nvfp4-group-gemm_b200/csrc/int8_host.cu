@@ -83,10 +83,14 @@ int int8_device(Int8Device** out, DeviceState** state) {
 int int8_ktiles(const nvfp4_int8_product* g) { return (g->k + kInt8StageK - 1) / kInt8StageK; }
 
 // What a product launches: one of NVFP4_INT8_*, the most tokens that a tile (or a pass over the
-// weights) takes, and the warps that share K or drain the accumulators.
+// weights) takes, the warps that share K or drain the accumulators, and the most tiles there can be.
 struct Int8Plan {
   int kernel, tokens, warps;
+  int64_t tiles;
 };
+Int8PairRows int8_pair_tile(int most) {
+  return {most, static_cast<uint32_t>(((int64_t{1} << 32) + most / 32 - 1) / (most / 32))};
+}
 
 // int8 rows [rows, k], `ld` bytes apart, in boxes of 128 bytes x box_rows, 128-byte swizzle,
 // zero fill past the last column and row.
@@ -117,6 +121,9 @@ bool int8_maps(const nvfp4_int8_product* g, int x_box, int w_box, Int8Maps* m) {
   return int8_map(&m->b2, g->b2, wrows, g->k, g->ldb, w_box);
 }
 
+// Most tiles of a launch: a persistent CTA's next tile number, the grid added to it, fits 31 bits.
+constexpr int64_t kInt8MaxTiles = 0x7fffffff - 65536;
+
 // The most tiles any segments can need: every row tile full, and one ragged tile each.
 int64_t int8_max_tiles(const nvfp4_int8_product* g, int tile_rows, int tile_n) {
   return ((g->rows + tile_rows - 1) / tile_rows + (g->num_experts - 1)) *
@@ -124,12 +131,11 @@ int64_t int8_max_tiles(const nvfp4_int8_product* g, int tile_rows, int tile_n) {
 }
 
 template <int TN, bool GATED>
-int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int num_sms, cudaStream_t s) {
+int launch_int8(const nvfp4_int8_product* g, const Int8GemmParams& p, int64_t tiles, int num_sms,
+                cudaStream_t s) {
   using Cfg = Int8Config<TN, GATED>;
   Int8Maps m;
   if (!int8_maps(g, TN, 128, &m)) return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
-  const int64_t tiles = int8_max_tiles(g, TN, 128);
-  if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
       launch_dependent(&nvfp4_int8_gemm_kernel<TN, GATED>, std::min<int64_t>(tiles, num_sms),
                        Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
@@ -170,19 +176,19 @@ int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p,
 }
 
 template <bool GATED, int WARPS>
-int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, int tile_rows, int clusters,
-                     cudaStream_t s) {
+int launch_int8_pair(const nvfp4_int8_product* g, Int8GemmParams p, const Int8Plan& plan,
+                     int clusters, cudaStream_t s) {
   using Cfg = Int8PairConfig<GATED, WARPS>;
   Int8Maps m;
-  p.pair_rows = tile_rows;
-  p.pair_inv = static_cast<uint32_t>(((int64_t{1} << 32) + tile_rows / 32 - 1) / (tile_rows / 32));
-  if (!int8_maps(g, tile_rows / 2, Cfg::kWBox, &m))
+  const Int8PairRows rows = int8_pair_tile(plan.tokens);
+  p.pair_rows = rows.most;
+  p.pair_inv = rows.inv;
+  if (!int8_maps(g, plan.tokens / 2, Cfg::kWBox, &m))
     return fail(NVFP4_ERR_DRIVER, "cuTensorMapEncodeTiled failed");
-  const int64_t tiles = int8_max_tiles(g, tile_rows, Cfg::kOutN);
-  if (tiles > 0x7fffffff) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   const cudaError_t e =
       launch_clusters(&nvfp4_int8_gemm_pair_kernel<GATED, WARPS>,
-                      std::min<int64_t>(tiles, clusters) * 2, 2, Cfg::kThreads, Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
+                      std::min<int64_t>(plan.tiles, clusters) * 2, 2, Cfg::kThreads,
+                      Cfg::kSmemBytes, s, m.a, m.a32, m.b, m.b2, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "int8 product launch");
 }
 
@@ -252,7 +258,7 @@ Int8Plan plan_int8(const nvfp4_int8_product* g, int num_sms, int clusters) {
     const int64_t groups = (static_cast<int64_t>(g->n) + r - 1) / r * active;
     int warps = 8;
     while (warps > 1 && (groups * warps > num_sms * 32 || g->k < 1024 * warps)) warps /= 2;
-    return Int8Plan{NVFP4_INT8_BYTES, tokens, warps};
+    return Int8Plan{NVFP4_INT8_BYTES, tokens, warps, 0};
   };
   // Experts' counts vary: twice the average, unless each is expected to have one row.
   const int64_t at_once = g->num_experts > 1 && rows > 1 ? 2 * rows : rows;
@@ -265,12 +271,13 @@ Int8Plan plan_int8(const nvfp4_int8_product* g, int num_sms, int clusters) {
   if (many && rows > 80 && (!gated || ktiles > 10)) {
     const int tile_rows = g->seg_offsets == nullptr ? int8_pair_rows(g, gated, ktiles, clusters)
                                                     : kInt8PairTokens;
-    return {NVFP4_INT8_PAIRS, tile_rows, ktiles <= (gated ? 18 : 8) ? 16 : 8};
+    return {NVFP4_INT8_PAIRS, tile_rows, ktiles <= (gated ? 18 : 8) ? 16 : 8,
+            int8_max_tiles(g, tile_rows, gated ? 128 : 256)};
   }
   auto fits = [&](int tn) { return many ? 4 * tn >= 5 * rows : one_wave(tn); };
   int tn = 16;
   while (tn < 128 && !fits(tn)) tn *= 2;
-  return {NVFP4_INT8_TILES, tn, tn >= 64 ? 8 : 4};
+  return {NVFP4_INT8_TILES, tn, tn >= 64 ? 8 : 4, int8_max_tiles(g, tn, 128)};
 }
 
 template <bool GATED>
@@ -284,12 +291,12 @@ int launch_plan_int8(const Int8Plan& plan, const nvfp4_int8_product* g, const In
            : tokens == 4 ? launch_int8_gemv_split<4, GATED>(g, p, plan.warps, sms, s)
                          : launch_int8_gemv_split<8, GATED>(g, p, plan.warps, sms, s);
   if (plan.kernel == NVFP4_INT8_PAIRS)
-    return plan.warps == 16 ? launch_int8_pair<GATED, 16>(g, p, tokens, ds.pair_clusters, s)
-                            : launch_int8_pair<GATED, 8>(g, p, tokens, ds.pair_clusters, s);
-  return tokens == 16   ? launch_int8<16, GATED>(g, p, sms, s)
-         : tokens == 32 ? launch_int8<32, GATED>(g, p, sms, s)
-         : tokens == 64 ? launch_int8<64, GATED>(g, p, sms, s)
-                        : launch_int8<128, GATED>(g, p, sms, s);
+    return plan.warps == 16 ? launch_int8_pair<GATED, 16>(g, p, plan, ds.pair_clusters, s)
+                            : launch_int8_pair<GATED, 8>(g, p, plan, ds.pair_clusters, s);
+  return tokens == 16   ? launch_int8<16, GATED>(g, p, plan.tiles, sms, s)
+         : tokens == 32 ? launch_int8<32, GATED>(g, p, plan.tiles, sms, s)
+         : tokens == 64 ? launch_int8<64, GATED>(g, p, plan.tiles, sms, s)
+                        : launch_int8<128, GATED>(g, p, plan.tiles, sms, s);
 }
 
 template <typename T, int G, int V>
@@ -436,9 +443,14 @@ NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* g, int num_sms, int cta_
   *launch = {};
   if (g->rows == 0) return NVFP4_OK;
   const Int8Plan plan = plan_int8(g, num_sms, cta_pairs);
+  if (plan.tiles > kInt8MaxTiles) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   launch->kernel = plan.kernel;
   launch->tokens = plan.tokens;
   launch->warps = plan.warps;
+  launch->rows = std::min<int64_t>(g->rows, plan.tokens);
+  if (plan.kernel == NVFP4_INT8_PAIRS)
+    launch->rows = int8_equal_rows(static_cast<int>(g->rows),
+                                   int8_pair_tile(plan.tokens).tiles(static_cast<int>(g->rows)));
   return NVFP4_OK;
 }
 
@@ -469,6 +481,7 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
                                                    : kInt8OutFp32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Int8Plan plan = plan_int8(g, ds->num_sms, ds->pair_clusters);
+  if (plan.tiles > kInt8MaxTiles) return fail(NVFP4_ERR_BAD_SHAPE, "too many tiles");
   return g->b2 != nullptr ? launch_plan_int8<true>(plan, g, p, *ds, s)
                           : launch_plan_int8<false>(plan, g, p, *ds, s);
 }

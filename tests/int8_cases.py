@@ -24,8 +24,8 @@ ONE_EXPERT_N = 410
 ONE_EXPERT = [(1, 1000, 1), (1, 2100, 2), (2, 1030, 1), (2, 4111, 4), (4, 1030, 1), (4, 8200, 8)]
 
 
-def plan(pkg, rows, n, k, experts=1, gated=False, expected=0, segments=False, sms=SMS, pairs=CTA_PAIRS):
-    """(kernel, tokens, warps) of a product of these sizes."""
+def launch(pkg, rows, n, k, experts=1, gated=False, expected=0, segments=False, sms=SMS, pairs=CTA_PAIRS):
+    """What a product of these sizes launches (nvfp4_int8_launch)."""
     N = pkg._native
     p = N.Int8Product(a=0x10000, b=0x20000, a_scale=0x30000, b_scale=0x40000, out=0x50000, rows=rows, n=n, k=k,
                       lda=(k + 15) // 16 * 16, ldb=(k + 15) // 16 * 16, ldo=n, num_experts=experts, out_dtype=0,
@@ -37,6 +37,12 @@ def plan(pkg, rows, n, k, experts=1, gated=False, expected=0, segments=False, sm
     got = N.Int8Launch()
     lib = pkg.load_library()
     N.check(lib.nvfp4_int8_plan(ctypes.byref(p), sms, pairs, ctypes.byref(got)), lib)
+    return got
+
+
+def plan(pkg, *args, **kw):
+    """(kernel, tokens, warps) of a product."""
+    got = launch(pkg, *args, **kw)
     return got.kernel, got.tokens, got.warps
 
 

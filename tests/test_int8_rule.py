@@ -50,3 +50,25 @@ def test_of_no_rows_and_refusals(pkg):
         C.plan(pkg, 4, 64, 131072)
     with pytest.raises(pkg.Nvfp4Error):
         C.plan(pkg, 4, 64, 64, sms=0)
+
+
+MOST_ROWS = 2 ** 31 - 1 - 256
+
+
+@pytest.mark.parametrize("rows", [MOST_ROWS, MOST_ROWS - 1, 2_139_127_681, 2_139_127_680, 2 ** 30, 193, 8192, 8193])
+def test_rows_of_a_tile_up_to_the_largest_count(pkg, rows):
+    """Equal tiles hold all rows, none more than the kernel's accumulators, for counts whose sum with the
+    number of tiles passes 2^31 as well."""
+    got = C.launch(pkg, rows, 20000, 16)
+    assert got.kernel == C.PAIRS
+    tiles = -(-rows // got.tokens)
+    assert got.rows % 32 == 0 and 0 < got.rows <= got.tokens <= 256
+    assert (tiles - 1) * got.rows < rows <= tiles * got.rows
+
+
+def test_tile_numbers_stay_below_2_to_31_with_a_stride_added(pkg):
+    """Persistent CTAs add the grid to a tile's number: the sum has to fit as well."""
+    rows, n = 2 ** 15 * 256, 65535 * 256
+    with pytest.raises(pkg.Nvfp4Error, match="too many tiles"):
+        C.launch(pkg, rows, n, 16)
+    assert C.launch(pkg, rows, n // 2, 16).kernel == C.PAIRS
