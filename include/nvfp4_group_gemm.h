@@ -299,12 +299,15 @@ NVFP4_API int nvfp4_moe_combine(const void* y, int64_t ldy, const int32_t* dest,
                                 const float* weights, int tokens, int topk, int cols, void* out,
                                 int64_t ldo, void* stream);
 
+#define NVFP4_MAX_ROW_COLUMNS (1 << 30) /* columns of the token sort and the int8 quantiser */
+
 /*
  * Tokens sorted by expert and back, with gradients (no counterpart in the reference, which is
  * inference only). dtype is NVFP4_DTYPE_BF16, _FP16 or _FP32 for every row argument; dest
  * [tokens * topk] and src_rows [rows] are nvfp4_moe_route's (pairs whose row is outside
  * [0, rows) are dropped pairs; every other row may be named by one pair only). Any column
- * count, alignment and row stride; rows on 16-byte boundaries move fastest.
+ * count up to NVFP4_MAX_ROW_COLUMNS, any alignment and row stride; rows on 16-byte boundaries
+ * move fastest.
  *   dispatch: y[dest[t, j]] = x[t]; zeros on the rows with src_rows[r] < 0
  *   combine:  out[t] = sum_j weights[t, j] * y[dest[t, j]] (fp32 products and sums in slot
  *             order, rounded once; weights NULL: ones). Without weights this is the gradient
@@ -329,7 +332,7 @@ NVFP4_API int nvfp4_moe_combine_tokens_backward(const void* grad_out, int64_t ld
 /*
  * int8 row quantiser (no counterpart in the reference): scales[r] = max_k |x[r, k]| / 127,
  * codes[r, k] = 127 * x[r, k] / max|x[r]| rounded to nearest, ties to even, of the exact
- * quotient. x bf16 or fp16 [rows, cols], any alignment and row stride ld (elements); codes
+ * quotient. x bf16 or fp16 [rows, cols <= NVFP4_MAX_ROW_COLUMNS], any alignment and row stride ld (elements); codes
  * int8, 16-byte aligned, row stride codes_ld a multiple of 16 bytes (bytes past cols are not
  * written). A row of zeros has scale 0; a row holding an infinity or a NaN has scale NaN and
  * zero codes. row_list (or NULL: every row): device int32 [listed], the rows to quantise, each in

@@ -332,7 +332,8 @@ int quantize_int8_impl(const void* x, int64_t rows, int cols, int64_t ld, int dt
                        void* codes, int64_t codes_ld, float* scales, void* stream) {
   if (dtype != NVFP4_DTYPE_BF16 && dtype != NVFP4_DTYPE_FP16)
     return fail(NVFP4_ERR_INVALID_ARGUMENT, "dtype=%d (expected NVFP4_DTYPE_BF16 or _FP16)", dtype);
-  if (rows < 0 || rows > 0x7fffffff || out_rows < 0 || out_rows > 0x7fffffff || cols <= 0)
+  if (rows < 0 || rows > 0x7fffffff || out_rows < 0 || out_rows > 0x7fffffff || cols <= 0 ||
+      cols > NVFP4_MAX_ROW_COLUMNS)
     return fail(NVFP4_ERR_BAD_SHAPE, "rows=%lld out_rows=%lld cols=%d", static_cast<long long>(rows),
                 static_cast<long long>(out_rows), cols);
   if (listed < 0 || listed > 0x7fffffff)

@@ -28,7 +28,9 @@ int check_sizes(int tokens, int topk, int cols, int64_t rows, int dtype, const v
   if (element_size(dtype) == 0)
     return fail(NVFP4_ERR_INVALID_ARGUMENT, "dtype=%d (expected NVFP4_DTYPE_BF16, _FP16 or _FP32)",
                 dtype);
-  if (tokens < 0 || topk <= 0 || cols <= 0 || rows < 0 || rows > 0x7fffffff - 32)
+  // The kernels' column counters step past the last column by as much as a block's span.
+  if (tokens < 0 || topk <= 0 || cols <= 0 || cols > NVFP4_MAX_ROW_COLUMNS || rows < 0 ||
+      rows > 0x7fffffff - 32)
     return fail(NVFP4_ERR_BAD_SHAPE, "tokens=%d topk=%d cols=%d rows=%lld", tokens, topk, cols,
                 static_cast<long long>(rows));
   if (static_cast<int64_t>(tokens) * topk > (int64_t{1} << 30))

@@ -120,3 +120,19 @@ def test_block_refuses_bad_sizes(pkg):
         pkg.moe.Int8MoEBlock(w, 0, 2)
     with pytest.raises(ValueError, match="dtype"):
         pkg.moe.Int8MoEBlock(w, 4, 2, dtype=torch.float32)
+
+
+WIDE = 2 ** 30 + 8  # columns past the operators' limit
+
+
+def test_columns_past_the_kernels_index_range(pkg):
+    """Column counters step past the last column by up to a block's span: counts near 2^31 are refused."""
+    lib = pkg.load_library()
+    for cols in (WIDE, 2 ** 31 - 1):
+        ld = (cols + 15) // 16 * 16
+        assert lib.nvfp4_quantize_int8(0x1000, 1, cols, ld, 0, None, 0, 0x2000, ld, 0x3000, None) == 2
+        assert lib.nvfp4_moe_dispatch_int8(0x1000, 1, cols, ld, 0, 0x4000, 1, 128, 0x2000, ld, 0x3000, None) == 2
+        assert lib.nvfp4_moe_dispatch_tokens(0x1000, ld, 0, 0x2000, 0x3000, 1, 1, cols, 128, 0x4000, ld, None) == 2
+        assert lib.nvfp4_moe_combine_tokens(0x1000, ld, 0, 0x2000, None, 1, 1, cols, 128, 0x4000, ld, None) == 2
+        assert lib.nvfp4_moe_combine_tokens_backward(0x1000, ld, 0x2000, ld, 0, 0x3000, 0x4000, None, 1, 1, cols, 128,
+                                                     0x5000, ld, 0x6000, None) == 2
