@@ -145,6 +145,11 @@ DTYPE_FP32 = 2
 # Limits of nvfp4_int8_gemm.
 INT8_MAX_EXPERTS = 1024
 INT8_MAX_K = 131071
+INT8_MAX_CHANNELS = 2 ** 31 - 257  # of all experts
+
+# Limits of the int8 quantiser and the token sort (NVFP4_MAX_ROW_COLUMNS; tokens times top-k).
+MAX_ROW_COLUMNS = 1 << 30
+MAX_PAIRS = 1 << 30
 
 # Largest group count nvfp4_grouped_gemm_noalloc accepts (NVFP4_NOALLOC_MAX_GROUPS).
 NOALLOC_MAX_GROUPS = 512

@@ -61,12 +61,16 @@ def _unit_inner(t: torch.Tensor) -> bool:
 
 
 def _check_activations(x: torch.Tensor) -> None:
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    if not isinstance(x, torch.Tensor):
         raise ValueError("x must be a CUDA tensor")
     if x.dtype not in _IN_DTYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if x.dim() != 2 or x.shape[1] < 1 or not _unit_inner(x):
         raise ValueError("x must be 2-D with unit stride along the last dimension")
+    if x.shape[1] > _native.MAX_ROW_COLUMNS:
+        raise ValueError(f"x has {x.shape[1]} columns, at most {_native.MAX_ROW_COLUMNS}")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         raise ValueError("rows of x must not overlap (expanded tensors: call .contiguous())")
 
@@ -198,6 +202,8 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     n = b.shape[0]
     if b.shape[1] != k or n < 1:
         raise ValueError(f"b must be [N >= 1, {k}], got {list(b.shape)}")
+    if n > _native.INT8_MAX_CHANNELS:
+        raise ValueError(f"b has {n} channels, at most {_native.INT8_MAX_CHANNELS}")
     if k > _native.INT8_MAX_K:
         raise ValueError(f"K={k} is above {_native.INT8_MAX_K}: sums could leave int32")
     _check_scale(a_scale, (m,), "a_scale")
@@ -253,6 +259,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     experts, n = int(b.shape[0]), int(b.shape[1])
     if experts > _native.INT8_MAX_EXPERTS:
         raise ValueError(f"at most {_native.INT8_MAX_EXPERTS} experts")
+    if experts * n > _native.INT8_MAX_CHANNELS:
+        raise ValueError(f"b has {experts * n} channels, at most {_native.INT8_MAX_CHANNELS}")
     if (b2 is None) != (b2_scale is None):
         raise ValueError("b2 and b2_scale must both be given")
     if b2 is not None:

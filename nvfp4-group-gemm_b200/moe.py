@@ -145,6 +145,8 @@ def dispatch_int8(x: torch.Tensor, routing: Routing, codes: torch.Tensor | None 
     """:func:`quantize_int8` of each token straight into its experts' rows: ``(codes, scales)``
     of ``routing.rows`` rows in dispatched order, each token read and quantised once. Padding
     rows are not written (the products do not read them either)."""
+    if routing.tokens * routing.topk > _native.MAX_PAIRS:
+        raise ValueError(f"{routing.tokens * routing.topk} pairs, at most {_native.MAX_PAIRS}")
     _check_activations(x)
     if int(x.shape[0]) != routing.tokens:
         raise ValueError(f"x must have {routing.tokens} rows, got {int(x.shape[0])}")

@@ -29,6 +29,8 @@ def _check_routing(routing) -> tuple:
     """``(tokens, topk, rows, dest, src_rows)`` of a Routing, checked against one another."""
     tokens, topk, rows = routing.tokens, routing.topk, routing.rows
     dest, src = routing.dest, routing.src_rows
+    if tokens * topk > _native.MAX_PAIRS:
+        raise ValueError(f"{tokens * topk} pairs, at most {_native.MAX_PAIRS}")
     if dest.dtype != torch.int32 or dest.numel() < tokens * topk or not dest.is_contiguous():
         raise ValueError(f"routing.dest must be contiguous int32 with {tokens * topk} entries")
     if src.dtype != torch.int32 or src.numel() < rows or not src.is_contiguous():
@@ -40,6 +42,8 @@ def _check_rows(t: torch.Tensor, rows: int, name: str, cols: int | None = None) 
     if not isinstance(t, torch.Tensor) or t.dtype not in _OUT_DTYPES or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D CUDA bf16, fp16 or fp32 tensor")
     have = t.shape
+    if have[1] > _native.MAX_ROW_COLUMNS:
+        raise ValueError(f"{name} has {have[1]} columns, at most {_native.MAX_ROW_COLUMNS}")
     if have[0] != rows or have[1] < 1 or (cols is not None and have[1] != cols):
         want = f"[{rows}, {'cols' if cols is None else cols}]"
         raise ValueError(f"{name} must be {want}, got {list(t.shape)}")

@@ -136,3 +136,36 @@ def test_columns_past_the_kernels_index_range(pkg):
         assert lib.nvfp4_moe_combine_tokens(0x1000, ld, 0, 0x2000, None, 1, 1, cols, 128, 0x4000, ld, None) == 2
         assert lib.nvfp4_moe_combine_tokens_backward(0x1000, ld, 0x2000, ld, 0, 0x3000, 0x4000, None, 1, 1, cols, 128,
                                                      0x5000, ld, 0x6000, None) == 2
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("cols", [WIDE, 2 ** 32 + 5])
+def test_python_refuses_wide_rows(pkg, cols):
+    """... and none is cut to its low 32 bits on the way."""
+    r = pkg.moe.Routing(1, 1, 1, [1], [0, 128], torch.zeros(1, dtype=torch.int32), torch.zeros(128, dtype=torch.int32))
+    for call in (lambda: pkg.quantize_int8(_meta(1, cols)), lambda: pkg.moe.dispatch_int8(_meta(1, cols), r),
+                 lambda: pkg.moe.dispatch_tokens(_meta(1, cols), r), lambda: pkg.moe.combine_tokens(_meta(128, cols), r),
+                 lambda: pkg.moe.dispatch_tokens_backward(_meta(128, cols), r),
+                 lambda: pkg.moe.combine_tokens_backward(_meta(1, cols), _meta(128, cols), r)):
+        with pytest.raises(ValueError, match="columns"):
+            call()
+
+
+def test_python_refuses_more_pairs_or_channels_than_32_bits_hold(pkg):
+    many = 2 ** 32 + 1
+    r = pkg.moe.Routing(many, 1, 1, [1], [0, 128], _meta(many, dtype=torch.int32), _meta(128, dtype=torch.int32))
+    for call in (lambda: pkg.moe.dispatch_tokens(_meta(many, 8), r), lambda: pkg.moe.combine_tokens(_meta(128, 8), r),
+                 lambda: pkg.moe.dispatch_int8(_meta(many, 8), r),
+                 lambda: pkg.moe.combine_tokens_backward(_meta(many, 8), _meta(128, 8), r)):
+        with pytest.raises(ValueError, match="pairs"):
+            call()
+    i8, f32 = dict(dtype=torch.int8), dict(dtype=torch.float32)
+    a, sa = _meta(4, 16, **i8), _meta(4, **f32)
+    with pytest.raises(ValueError, match="channels"):
+        pkg.int8_gemm(a, sa, _meta(2 ** 31, 16, **i8), _meta(2 ** 31, **f32))
+    with pytest.raises(ValueError, match="channels"):
+        pkg.int8_gemm_segments(a, sa, _meta(4, 2 ** 29, 16, **i8), _meta(4, 2 ** 29, **f32),
+                               torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
