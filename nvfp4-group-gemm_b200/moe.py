@@ -569,8 +569,13 @@ class Int8MoEBlock:
 
     def run(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
             stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-        """One block on ``stream``."""
+        """One block on ``stream``; inputs and buffers are recorded there where it is not the
+        current one, so that freeing them after the call does not hand their memory out early."""
         self._check_inputs(x, topk_ids, topk_weights)
+        if stream is not None:
+            _launch_on((x, topk_ids, topk_weights, self._meta, self.dest, self.src_rows,
+                        self._route_ws, self._a, self._a_scale, self._h, self._a2, self._a2_scale,
+                        self._y, self._w, self.out), stream)
         st = stream or torch.cuda.current_stream(self.device)
         s = st.cuda_stream
         lib, chk = self._lib, _native.check
