@@ -36,7 +36,7 @@ extern "C" {
 /* 3: int8 products (nvfp4_int8_gemm, nvfp4_quantize_int8, nvfp4_moe_dispatch_int8), token sort
  * with gradients (nvfp4_moe_dispatch_tokens, nvfp4_moe_combine_tokens and its backward),
  * NVFP4_DTYPE_FP32. */
-/* 4: nvfp4_int8_plan. */
+/* 4: nvfp4_int8_plan, error words of the caller's for int8 products. */
 #define NVFP4_ABI_VERSION 4
 
 typedef enum nvfp4_status {
@@ -363,8 +363,8 @@ NVFP4_API int nvfp4_moe_dispatch_int8(const void* x, int tokens, int cols, int64
  * expected_rows (0: rows) is the host's estimate of the rows in all segments; it picks the
  * tile shape only. bias needs one expert and no b2. num_experts <= 1024.
  *
- * Needs no workspace and keeps nothing between calls: calls may overlap on any streams and in
- * any CUDA graphs.
+ * Needs no workspace and keeps nothing between calls but what nvfp4_int8_check reports: calls may
+ * overlap on any streams and in any CUDA graphs.
  */
 typedef struct nvfp4_int8_product {
   const void* a;
@@ -409,11 +409,22 @@ NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* product, int num_sms, in
                               nvfp4_int8_launch* launch);
 
 /*
+ * The same with an error word of the caller's (device memory, zero at first), which must live as
+ * long as the call and any graph that holds it. NULL: the device's word, as nvfp4_int8_gemm.
+ */
+NVFP4_API int nvfp4_int8_gemm_reporting(const nvfp4_int8_product* product,
+                                        unsigned int* error_word, void* stream);
+
+/*
  * Synchronise `stream`, then read and clear the current device's error word of the int8
  * products: NVFP4_ERR_DEVICE_TIMEOUT when a kernel gave up on a wait, NVFP4_ERR_BAD_SHAPE when
- * a segment was outside its slab (skipped).
+ * a segment was outside its slab (skipped). Every caller without a word of its own shares this
+ * one: the report may be of another's product, and is gone for that caller.
+ * nvfp4_int8_check_word: the same of a caller's word (NULL: the device's).
  */
 NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits);
+NVFP4_API int nvfp4_int8_check_word(unsigned int* error_word, void* stream,
+                                    unsigned int* device_error_bits);
 
 /*
  * Expert-parallel MoE exchange over NVLink peer memory: one process per GPU, `world` ranks

@@ -87,7 +87,9 @@ EXPORTED_SYMBOLS = (
     "nvfp4_moe_dispatch_int8",
     "nvfp4_int8_gemm",
     "nvfp4_int8_plan",
+    "nvfp4_int8_gemm_reporting",
     "nvfp4_int8_check",
+    "nvfp4_int8_check_word",
 )
 
 ABI_VERSION = 4   # NVFP4_ABI_VERSION
@@ -355,6 +357,10 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         lib.nvfp4_moe_dispatch_int8.restype = i32
         lib.nvfp4_int8_gemm.argtypes = [vp, vp]
         lib.nvfp4_int8_gemm.restype = i32
+        lib.nvfp4_int8_gemm_reporting.argtypes = [vp, vp, vp]
+        lib.nvfp4_int8_gemm_reporting.restype = i32
+        lib.nvfp4_int8_check_word.argtypes = [vp, vp, ctypes.POINTER(ctypes.c_uint)]
+        lib.nvfp4_int8_check_word.restype = i32
         lib.nvfp4_int8_plan.argtypes = [vp, i32, i32, ctypes.POINTER(Int8Launch)]
         lib.nvfp4_int8_plan.restype = i32
         lib.nvfp4_int8_check.argtypes = [vp, ctypes.POINTER(ctypes.c_uint)]

@@ -15,10 +15,18 @@
 
 namespace nvfp4 {
 
-// Why a product gave up on a wait or skipped a segment (kDevErr* bits), one word per device.
-// A product needs no workspace: its tensor maps travel as kernel parameters and nothing of one
-// call is left for the next, so calls on any streams and in any graphs may overlap.
+// Why a product gave up on a wait or skipped a segment (kDevErr* bits): in the caller's word, or
+// in this one of the device, which all callers without a word of their own share.
+// A product needs no workspace: its tensor maps travel as kernel parameters and nothing else of
+// one call is left for the next, so calls on any streams and in any graphs may overlap.
 __device__ uint32_t g_int8_error_bits;
+
+// Reads and clears an error word in one step: bits that another stream sets meanwhile are in this
+// report or in the next.
+__device__ uint32_t g_int8_taken_bits;
+__global__ void nvfp4_int8_take_errors_kernel(uint32_t* word) {
+  g_int8_taken_bits = atomicExch(word, 0u);
+}
 
 namespace {
 
@@ -26,6 +34,8 @@ struct Int8Device {
   std::once_flag once;
   cudaError_t status = cudaSuccess;
   uint32_t* error_bits = nullptr;
+  uint32_t* taken_bits = nullptr;
+  std::mutex taking;  // one check at a time uses taken_bits
 };
 Int8Device g_int8_dev[kMaxDevices];
 
@@ -61,6 +71,8 @@ void init_int8_device(Int8Device& d) {
   void* p = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&p, g_int8_error_bits);
   d.error_bits = static_cast<uint32_t*>(p);
+  if (e == cudaSuccess) e = cudaGetSymbolAddress(&p, g_int8_taken_bits);
+  d.taken_bits = static_cast<uint32_t*>(p);
   if (e == cudaSuccess) e = allow_smem_all<false>();
   if (e == cudaSuccess) e = allow_smem_all<true>();
   d.status = e;
@@ -456,6 +468,11 @@ NVFP4_API int nvfp4_int8_plan(const nvfp4_int8_product* g, int num_sms, int cta_
 }
 
 NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
+  return nvfp4_int8_gemm_reporting(g, nullptr, stream);
+}
+
+NVFP4_API int nvfp4_int8_gemm_reporting(const nvfp4_int8_product* g, unsigned int* error_word,
+                                        void* stream) {
   g_last_error.clear();
   const int bad = check_product(g);
   if (bad != NVFP4_OK || g->rows == 0) return bad;
@@ -472,7 +489,7 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
   p.ldo = g->ldo;
   p.seg_offsets = g->seg_offsets;
   p.seg_counts = g->seg_counts;
-  p.error_bits = d->error_bits;
+  p.error_bits = error_word != nullptr ? error_word : d->error_bits;
   p.rows = static_cast<int32_t>(g->rows);
   p.n = g->n;
   p.ktiles = int8_ktiles(g);
@@ -488,13 +505,39 @@ NVFP4_API int nvfp4_int8_gemm(const nvfp4_int8_product* g, void* stream) {
 }
 
 NVFP4_API int nvfp4_int8_check(void* stream, unsigned int* device_error_bits) {
+  return nvfp4_int8_check_word(nullptr, stream, device_error_bits);
+}
+
+NVFP4_API int nvfp4_int8_check_word(unsigned int* error_word, void* stream,
+                                    unsigned int* device_error_bits) {
   g_last_error.clear();
   if (device_error_bits) *device_error_bits = 0;
   Int8Device* d = nullptr;
   DeviceState* ds = nullptr;
   const int st = int8_device(&d, &ds);
   if (st != NVFP4_OK) return st;
-  return nvfp4_workspace_check(d->error_bits, stream, device_error_bits);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamSynchronize");
+  uint32_t bits = 0;
+  {
+    std::lock_guard<std::mutex> lock(d->taking);
+    nvfp4_int8_take_errors_kernel<<<1, 1, 0, s>>>(error_word != nullptr ? error_word
+                                                                        : d->error_bits);
+    e = cudaGetLastError();
+    if (e == cudaSuccess)
+      e = cudaMemcpyAsync(&bits, d->taken_bits, sizeof(bits), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "read error word");
+  if (device_error_bits) *device_error_bits = bits;
+  if (bits & kDevErrTimeouts)
+    return fail(NVFP4_ERR_DEVICE_TIMEOUT, "device error bits 0x%x", bits);
+  if (bits != 0)
+    return fail(NVFP4_ERR_BAD_SHAPE,
+                "device error bits 0x%x: a device-side row segment was out of range (skipped)",
+                bits);
+  return NVFP4_OK;
 }
 
 }  // extern "C"

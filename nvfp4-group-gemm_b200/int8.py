@@ -7,8 +7,9 @@ codes with scales per token and per channel, dense or over the rows of every exp
 
 Code matrices are int8 with unit inner stride and rows a multiple of 16 bytes apart, which is
 how :func:`quantize_int8` allocates them for any number of columns. The products need no
-workspace and keep nothing between calls, so calls may overlap on any streams and be captured
-in any CUDA graphs. The reference has no 8-bit form of its product.
+workspace and keep nothing between calls but their errors, so calls may overlap on any streams
+and be captured in any CUDA graphs. Errors go to one word per GPU, which all calls share, or to
+an ``error_word`` of the caller's. The reference has no 8-bit form of its product.
 """
 from __future__ import annotations
 
@@ -91,6 +92,11 @@ def _codes_stride(t: torch.Tensor, name: str) -> int:
     return ld
 
 
+def _check_word(t) -> None:
+    if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.numel() != 1):
+        raise ValueError("error_word must be a CUDA int32 tensor of one entry (zero at first)")
+
+
 def _check_scale(t: torch.Tensor, shape: tuple, name: str) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != shape or \
             not t.is_contiguous():
@@ -165,7 +171,7 @@ def _check_out(out, out_dtype, rows: int, n: int) -> None:
 
 
 def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, out_dtype, n, k, experts,
-             offsets, counts, expected_rows, raw):
+             offsets, counts, expected_rows, error_word, raw):
     rows = a.shape[0]
     if out is None:
         dtype = torch.bfloat16 if out_dtype is None else out_dtype
@@ -182,21 +188,24 @@ def _product(a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, bias, out, out_dtyp
         counts.data_ptr() if counts is not None else 0, rows, lda, ldb, ldo, expected_rows, n, k,
         experts, _OUT_DTYPES[dtype])
     lib = _native.load_library()
-    _native.check(lib.nvfp4_int8_gemm(product, raw), lib)
+    word = error_word.data_ptr() if error_word is not None else None
+    _native.check(lib.nvfp4_int8_gemm_reporting(product, word, raw), lib)
     return out
 
 
 def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
               bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
-              out_dtype: torch.dtype | None = None,
-              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+              out_dtype: torch.dtype | None = None, stream: torch.cuda.Stream | None = None,
+              error_word: torch.Tensor | None = None) -> torch.Tensor:
     """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k] (+ bias[n])``.
 
     ``a`` int8 [M, K] (codes of tokens), ``b`` int8 [N, K] (codes of weight rows), scales fp32
     [M] and [N], ``bias`` fp32 [N]. The sums are exact; the result is rounded once, to
     ``out_dtype`` (bf16 by default; fp16, fp32). Any M, N and K up to 131071; ``out`` may have
-    any row stride and alignment.
+    any row stride and alignment. ``error_word``: where a wait that timed out is reported (see
+    :func:`check_int8_errors`).
     """
+    _check_word(error_word)
     lda, ldb = _codes_stride(a, "a"), _codes_stride(b, "b")
     m, k = a.shape
     n = b.shape[0]
@@ -211,9 +220,9 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     if bias is not None:
         _check_scale(bias, (n,), "bias")
     _check_out(out, out_dtype, m, n)
-    raw, where = _launch_on((a, a_scale, b, b_scale, bias, out), stream)
+    raw, where = _launch_on((a, a_scale, b, b_scale, bias, out, error_word), stream)
     return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, None, None, bias, out,
-                   out_dtype, n, k, 1, None, None, 0, raw)
+                   out_dtype, n, k, 1, None, None, 0, error_word, raw)
 
 
 def _expert_weights(b: torch.Tensor, b_scale: torch.Tensor, k: int, name: str) -> int:
@@ -236,7 +245,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
                        seg_counts: torch.Tensor, b2: torch.Tensor | None = None,
                        b2_scale: torch.Tensor | None = None, out: torch.Tensor | None = None,
                        out_dtype: torch.dtype | None = None, expected_rows: int = 0,
-                       stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+                       stream: torch.cuda.Stream | None = None,
+                       error_word: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`int8_gemm` over row segments of one slab, read on the GPU.
 
     ``a`` int8 [R, K] with scales [R]; expert e multiplies rows ``[seg_offsets[e],
@@ -249,8 +259,11 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     outside the slab is skipped and :func:`check_int8_errors` raises; segments that share rows
     are not supported (their rows hold either result; segments past the slab's number of rows in
     all may be skipped and reported). ``expected_rows`` (the host's estimate of all segments'
-    rows, e.g. tokens x top-k) picks the tile shape only.
+    rows, e.g. tokens x top-k) picks the tile shape only. ``error_word`` (int32 CUDA tensor of one
+    entry, zero at first; it has to outlive the call and any graph that holds it) takes the reports
+    in place of the device's word, which all other calls share.
     """
+    _check_word(error_word)
     lda = _codes_stride(a, "a")
     rows, k = int(a.shape[0]), int(a.shape[1])
     if k > _native.INT8_MAX_K:
@@ -271,22 +284,32 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
         if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.numel() < experts:
             raise ValueError(f"{name} must be a contiguous CUDA int32 tensor of >= {experts} entries")
     _check_out(out, out_dtype, rows, n)
-    raw, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out),
-                            stream)
+    raw, where = _launch_on((a, a_scale, b, b_scale, b2, b2_scale, seg_offsets, seg_counts, out,
+                             error_word), stream)
     return _within(where, _product, a, lda, a_scale, b, ldb, b_scale, b2, b2_scale, None, out,
-                   out_dtype, n, k, experts, seg_offsets, seg_counts, int(expected_rows), raw)
+                   out_dtype, n, k, experts, seg_offsets, seg_counts, int(expected_rows),
+                   error_word, raw)
 
 
 def check_int8_errors(device: torch.device | int | None = None,
-                      stream: torch.cuda.Stream | None = None) -> int:
-    """Synchronise ``stream`` (the current one by default) and read and clear the device error
-    bits of the int8 products: raises Nvfp4Error when a segment was out of range or a wait timed
-    out, else returns 0."""
+                      stream: torch.cuda.Stream | None = None,
+                      error_word: torch.Tensor | None = None) -> int:
+    """Synchronise ``stream`` (the current one by default) and read and clear, in one step, the
+    error bits of the int8 products in ``error_word``: raises Nvfp4Error when a segment was out of
+    range or a wait timed out, else returns 0. Without ``error_word``: the device's, of all calls
+    that were given none (whoever made them)."""
+    _check_word(error_word)
+    if error_word is not None:
+        if not error_word.is_cuda:
+            raise ValueError("error_word must be on a CUDA device")
+        device = error_word.device
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else \
         torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
     s = stream or torch.cuda.current_stream(dev)
     lib = _native.load_library()
     bits = ctypes.c_uint(0)
     with torch.cuda.device(dev):
-        _native.check(lib.nvfp4_int8_check(s.cuda_stream, ctypes.byref(bits)), lib)
+        _native.check(lib.nvfp4_int8_check_word(
+            error_word.data_ptr() if error_word is not None else None, s.cuda_stream,
+            ctypes.byref(bits)), lib)
     return int(bits.value)

@@ -554,6 +554,8 @@ class Int8MoEBlock:
         self._y = torch.empty((cap, hdim), dtype=dtype, device=dev)
         self._w = torch.empty((tokens, topk), **f32)
         self.out = torch.empty((tokens, hdim), dtype=dtype, device=dev)
+        self._errors = torch.zeros(1, **i32)  # of this block's products
+        self._last = None                     # the stream of the last run
         self._weights = weights
 
     def _check_inputs(self, x, topk_ids, topk_weights):
@@ -576,7 +578,7 @@ class Int8MoEBlock:
             _launch_on((x, topk_ids, topk_weights, self._meta, self.dest, self.src_rows,
                         self._route_ws, self._a, self._a_scale, self._h, self._a2, self._a2_scale,
                         self._y, self._w, self.out), stream)
-        st = stream or torch.cuda.current_stream(self.device)
+        st = self._last = stream or torch.cuda.current_stream(self.device)
         s = st.cuda_stream
         lib, chk = self._lib, _native.check
         T, K, E, cap, W = self.tokens, self.topk, self.num_experts, self.capacity, self._weights
@@ -591,10 +593,11 @@ class Int8MoEBlock:
                                             self._a_scale.data_ptr(), s), lib)
             int8_gemm_segments(self._a, self._a_scale, W.w_gate, W.s_gate, self.offsets, self.counts,
                                b2=W.w_up, b2_scale=W.s_up, out=self._h, expected_rows=T * K,
-                               stream=st)
+                               stream=st, error_word=self._errors)
             quantize_int8(self._h, self._a2, self._a2_scale, row_list=self.dest, stream=st)
             int8_gemm_segments(self._a2, self._a2_scale, W.w_down, W.s_down, self.offsets,
-                               self.counts, out=self._y, expected_rows=T * K, stream=st)
+                               self.counts, out=self._y, expected_rows=T * K, stream=st,
+                               error_word=self._errors)
             w = topk_weights
             if w.dtype != torch.float32 or not w.is_contiguous():
                 with torch.cuda.stream(st):
@@ -606,10 +609,13 @@ class Int8MoEBlock:
                                              self.out.data_ptr(), self.out.stride(0), s), lib)
         return self.out
 
-    def check_device_errors(self) -> int:
-        """Synchronise and return the device error bits of the int8 products (raises Nvfp4Error
-        when a segment was out of range or a wait timed out)."""
-        return check_int8_errors(self.device)
+    def check_device_errors(self, stream: torch.cuda.Stream | None = None) -> int:
+        """Synchronise the stream of the last run and ``stream`` (the current one by default; the
+        one that replays a captured run) and return the error bits of this block's products, which
+        it has to itself (raises Nvfp4Error when a segment was out of range or a wait timed out)."""
+        if self._last is not None:
+            self._last.synchronize()
+        return check_int8_errors(stream=stream, error_word=self._errors)
 
     def capture(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
                 warmup: int = 1) -> torch.cuda.CUDAGraph:

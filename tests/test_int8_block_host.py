@@ -54,7 +54,7 @@ def _block(pkg, monkeypatch, tokens=3, topk=2, E=4, hidden=16, inter=8):
                                ("_a_scale", (cap,), torch.float32), ("_h", (cap, inter), bf),
                                ("_a2", (cap, 16), torch.int8), ("_a2_scale", (cap,), torch.float32),
                                ("_y", (cap, hidden), bf), ("_w", (tokens, topk), torch.float32),
-                               ("out", (tokens, hidden), bf)):
+                               ("out", (tokens, hidden), bf), ("_errors", (1,), i32)):
         setattr(blk, name, _Tensor(shape, dtype))
     blk._route_ws_bytes = 64
     blk._weights = types.SimpleNamespace(**{k: _Tensor((E, 8, 16), torch.int8) for k in (

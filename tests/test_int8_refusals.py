@@ -169,3 +169,15 @@ def test_python_refuses_more_pairs_or_channels_than_32_bits_hold(pkg):
     with pytest.raises(ValueError, match="channels"):
         pkg.int8_gemm_segments(a, sa, _meta(4, 2 ** 29, 16, **i8), _meta(4, 2 ** 29, **f32),
                                torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+
+
+def test_error_words_are_checked(pkg):
+    q, s = torch.zeros((4, 32), dtype=torch.int8), torch.zeros(4)
+    for word in (torch.zeros(2, dtype=torch.int32), torch.zeros(1), 5):
+        for call in (lambda: pkg.int8_gemm(q, s, q, s, error_word=word),
+                     lambda: pkg.int8_gemm_segments(q, s, q[None], s[None], s.int(), s.int(), error_word=word),
+                     lambda: pkg.check_int8_errors(error_word=word)):
+            with pytest.raises(ValueError, match="error_word"):
+                call()
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.check_int8_errors(error_word=torch.zeros(1, dtype=torch.int32))
