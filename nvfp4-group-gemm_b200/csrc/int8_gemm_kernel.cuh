@@ -91,8 +91,11 @@ __device__ __forceinline__ void int8_store_rows(const Int8GemmParams& p, int64_t
     int8_store_rows_as(static_cast<float*>(p.out) + at, p.ldo, y, count);
 }
 
+// g / (1 + exp(-g)) * u. With e = exp(-|g|) the divisor lies in [1, 2]: written with exp(-g) it
+// passes 2^126 for g in (-88.7, -87.3), where the fast division returns 0.
 __device__ __forceinline__ float int8_silu_mul(float g, float u) {
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
+  const float e = __expf(-fabsf(g));
+  return __fdividef(g < 0.0f ? g * e : g, 1.0f + e) * u;
 }
 
 // Most token rows of a tile, and the tiles that hold `count` rows. Of CTA pairs these rows are the

@@ -33,3 +33,38 @@ def test_byte_products_of_one_expert(pkg, rows, k, warps):
     for count in (rows, 2 * rows + 1):
         T._segments_case(pkg, [2], [count], count + 5, C.ONE_EXPERT_N, k, True, torch.float16, rows, seed=k)
     assert pkg.check_int8_errors() == 0
+
+
+def _gated(pkg, rows, n, k, gate, up, dtype):
+    """One expert whose gate and up sums are exactly `gate` (a multiple of 1/64 above -129) and `up`
+    (a power of two) in every row; the output, and the kernel that made it."""
+    a = torch.zeros((rows, (k + 15) // 16 * 16), dtype=torch.int8)
+    a[:, 0], a[:, 1] = 64, 1
+    s = (gate * 64).round().long()
+    hi = torch.div(s, 64, rounding_mode="floor")
+    w = [torch.zeros((1, n, (k + 15) // 16 * 16), dtype=torch.int8) for _ in range(2)]
+    w[0][0, :, 0], w[0][0, :, 1] = hi.to(torch.int8), (s - 64 * hi).to(torch.int8)
+    w[1][0, :, 1] = 1
+    one = torch.ones(rows, device="cuda")
+    sw = [torch.full((1, n), v, device="cuda") for v in (1 / 64, up)]
+    off, cnt = (torch.tensor([v], dtype=torch.int32, device="cuda") for v in (0, rows))
+    out = pkg.int8_gemm_segments(a.cuda()[:, :k], one, w[0].cuda()[:, :, :k], sw[0], off, cnt, b2=w[1].cuda()[:, :, :k],
+                                 b2_scale=sw[1], out_dtype=dtype, expected_rows=rows)
+    return out.double().cpu(), C.plan(pkg, rows, n, k, 1, True, rows, True)[0]
+
+
+GATED_OF_EACH_KERNEL = [(1, 300, 64, C.BYTES), (130, 300, 64, C.TILES), (600, 5000, 1300, C.PAIRS)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,n,k,kernel", GATED_OF_EACH_KERNEL)
+def test_gates_whose_exponential_is_next_to_the_largest_float(pkg, rows, n, k, kernel, dtype):
+    """silu of -88.7 .. -87.3: exp(-g) is finite but above 2^126. With a large up sum the result is an
+    ordinary number. Tolerance: as in test_gpu_int8.py, and half a step of the subnormal exp(g) (at
+    most 2^-150 / 3e-39 = 4 u)."""
+    gate = -87.3125 - torch.arange(n).remainder(90).double() / 64
+    got, used = _gated(pkg, rows, n, k, gate, 2.0 ** 40, dtype)
+    assert used == kernel
+    want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 40).expand(rows, n)
+    tol = ((20 + 5.4 * 88.8) * T.U + T.HALF[dtype]) * want.abs()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / want.abs()).max())
