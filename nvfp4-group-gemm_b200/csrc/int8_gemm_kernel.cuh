@@ -92,10 +92,26 @@ __device__ __forceinline__ void int8_store_rows(const Int8GemmParams& p, int64_t
 }
 
 // g / (1 + exp(-g)) * u. With e = exp(-|g|) the divisor lies in [1, 2]: written with exp(-g) it
-// passes 2^126 for g in (-88.7, -87.3), where the fast division returns 0.
+// passes 2^126 for g in (-88.7, -87.3), where the fast division returns 0. FULL, for outputs of 32
+// bits, is within 8 * 2^-24; otherwise the fast exponential and division are taken, within
+// (5 + 1.2 |g|) * 2^-23, far below the rounding to 16 bits that follows.
+template <bool FULL>
 __device__ __forceinline__ float int8_silu_mul(float g, float u) {
-  const float e = __expf(-fabsf(g));
-  return __fdividef(g < 0.0f ? g * e : g, 1.0f + e) * u;
+  const float e = FULL ? expf(-fabsf(g)) : __expf(-fabsf(g));
+  const float x = g < 0.0f ? g * e : g;
+  return (FULL ? __fdiv_rn(x, 1.0f + e) : __fdividef(x, 1.0f + e)) * u;
+}
+// y[i] = silu(g[i]) * u[i]
+template <int M>
+__device__ __forceinline__ void int8_gate(int out_dtype, const float (&g)[M], const float (&u)[M],
+                                          float (&y)[M]) {
+  if (out_dtype == kInt8OutFp32) {
+#pragma unroll
+    for (int i = 0; i < M; ++i) y[i] = int8_silu_mul<true>(g[i], u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < M; ++i) y[i] = int8_silu_mul<false>(g[i], u[i]);
+  }
 }
 
 // Most token rows of a tile, and the tiles that hold `count` rows. Of CTA pairs these rows are the
@@ -407,10 +423,8 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
         const int tok = tok0 + 32 * i + lane;
         as[i] = tok < t.rows ? __ldg(p.a_scale + t.row + tok) : 0.0f;
       }
-      auto value = [&](int32_t g, int32_t w, float a) {
-        const float y = __fmul_rn(__fmul_rn(__int2float_rn(g), a), bs);
-        return GATED ? int8_silu_mul(y, __fmul_rn(__fmul_rn(__int2float_rn(w), a), bs2))
-                     : __fadd_rn(y, bias);
+      auto scaled = [](uint32_t sum, float a, float b) {
+        return __fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(sum)), a), b);
       };
       const int acc = static_cast<int>(local & 1u);
       if (!warp_wait_phase(&accf_bar[acc], (full_parity >> acc) & 1u, abort_flag, p.error_bits,
@@ -433,11 +447,15 @@ __global__ void __launch_bounds__(Int8Config<TN, GATED>::kThreads, 1)
         if (c >= toks) break;  // uniform over the warp
         uint32_t v[16], u[16];
         load16(c, v, u);
-        float y[16];
+        float y[16], w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          y[i] = value(static_cast<int32_t>(v[i]), GATED ? static_cast<int32_t>(u[i]) : 0,
-                       __shfl_sync(0xffffffffu, as[c / 32], (c + i) & 31));
+        for (int i = 0; i < 16; ++i) {
+          const float a = __shfl_sync(0xffffffffu, as[c / 32], (c + i) & 31);
+          y[i] = scaled(v[i], a, bs);
+          if (GATED) w[i] = scaled(u[i], a, bs2);
+          else y[i] = __fadd_rn(y[i], bias);
+        }
+        if constexpr (GATED) int8_gate(p.out_dtype, y, w, y);
         int8_store_rows(p, static_cast<int64_t>(t.row) + tok0 + c, n, y, toks - c);
       }
       ptx::tcgen05_fence_before_sync();

@@ -290,12 +290,14 @@ __global__ void __launch_bounds__(64 + 32 * WARPS, 1)
             break;
           }
           ++swaps;
-          float z[8];
+          float g[8], w[8], z[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float other = from[32 * i];
-            z[i] = up ? int8_silu_mul(other, y[8 + i]) : int8_silu_mul(y[i], other);
+            g[i] = up ? other : y[i];
+            w[i] = up ? y[8 + i] : other;
           }
+          int8_gate(p.out_dtype, g, w, z);
           const int first8 = tok + (up ? 8 : 0);
           int8_store_rows(p, static_cast<int64_t>(t.row) + first8, n, z, t.rows - first8);
         }

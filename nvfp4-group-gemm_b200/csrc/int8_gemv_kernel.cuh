@@ -173,11 +173,16 @@ __global__ void __launch_bounds__(kInt8GemvThreads, TB <= 4 ? 4 : 2)
         const int64_t chan = static_cast<int64_t>(e) * p.n + n;
         const float as = __ldg(p.a_scale + row);
         float y = __fmul_rn(__fmul_rn(__int2float_rn(sum), as), __ldg(p.b_scale + chan));
-        if (GATED)
-          y = int8_silu_mul(y, __fmul_rn(__fmul_rn(__int2float_rn(h), as),
-                                         __ldg(p.b2_scale + chan)));
-        else
+        if (GATED) {
+          const float g[1] = {y};
+          const float u[1] = {__fmul_rn(__fmul_rn(__int2float_rn(h), as),
+                                        __ldg(p.b2_scale + chan))};
+          float z[1];
+          int8_gate(p.out_dtype, g, u, z);
+          y = z[0];
+        } else {
           y = __fadd_rn(y, p.bias != nullptr ? __ldg(p.bias + n) : 0.0f);
+        }
         const int64_t at = row * p.ldo + n;
         if (p.out_dtype == kInt8OutBf16)
           static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);

@@ -68,3 +68,15 @@ def test_gates_whose_exponential_is_next_to_the_largest_float(pkg, rows, n, k, k
     want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 40).expand(rows, n)
     tol = ((20 + 5.4 * 88.8) * T.U + T.HALF[dtype]) * want.abs()
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / want.abs()).max())
+
+
+@pytest.mark.parametrize("rows,n,k,kernel", GATED_OF_EACH_KERNEL)
+def test_gated_fp32_outputs_have_32_bits(pkg, rows, n, k, kernel):
+    """Gate and up sums are exact here, so what is left is silu's own error. e = exp(-|g|) within 2 ulp
+    (4 u), g e, 1 + e and the quotient within half an ulp each (u); the up sum is a power of two: 7 u."""
+    gate = -80 + (torch.arange(n).double() * (160 * 64) / n).floor() / 64
+    got, used = _gated(pkg, rows, n, k, gate, 2.0 ** 10, torch.float32)
+    assert used == kernel
+    want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 10).expand(rows, n)
+    err = (got - want).abs()
+    assert bool((err <= 7 * T.U * want.abs()).all()), float((err / want.abs()).nan_to_num(0).max() / T.U)
