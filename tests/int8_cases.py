@@ -23,6 +23,13 @@ EIGHT_ROWS = [(False, 2048, 2), (False, 4111, 4), (False, 8200, 8), (True, 2100,
 ONE_EXPERT_N = 410
 ONE_EXPERT = [(1, 1000, 1), (1, 2100, 2), (2, 1030, 1), (2, 4111, 4), (4, 1030, 1), (4, 8200, 8)]
 
+# Gated products of one weight pair without segments (the C entry): (rows, n, k, kernel, tokens, warps).
+DENSE_GATED = [(1, 410, 1000, BYTES, 1, 1), (2, 410, 2100, BYTES, 2, 2), (4, 410, 1030, BYTES, 4, 1),
+               (7, 410, 4111, BYTES, 8, 4), (7, 2050, 300, TILES, 16, 4), (60, 5000, 200, TILES, 32, 4),
+               (102, 4778, 1300, TILES, 64, 8), (275, 3725, 1300, TILES, 128, 8), (93, 19500, 1290, PAIRS, 96, 16),
+               (971, 3084, 2011, PAIRS, 128, 16), (389, 4747, 1281, PAIRS, 160, 16), (487, 4772, 2400, PAIRS, 192, 8),
+               (804, 3728, 2305, PAIRS, 224, 8), (693, 4789, 1300, PAIRS, 256, 16)]
+
 
 def launch(pkg, rows, n, k, experts=1, gated=False, expected=0, segments=False, sms=SMS, pairs=CTA_PAIRS):
     """What a product of these sizes launches (nvfp4_int8_launch)."""

@@ -2,6 +2,9 @@
 64-bit restatements (tolerances: test_gpu_int8.py)."""
 from __future__ import annotations
 
+import ctypes
+
+import numpy as np
 import pytest
 import torch
 
@@ -80,3 +83,27 @@ def test_gated_fp32_outputs_have_32_bits(pkg, rows, n, k, kernel):
     want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 10).expand(rows, n)
     err = (got - want).abs()
     assert bool((err <= 7 * T.U * want.abs()).all()), float((err / want.abs()).nan_to_num(0).max() / T.U)
+
+
+@pytest.mark.parametrize("rows,n,k,kernel,tokens,warps", C.DENSE_GATED)
+def test_dense_gated_products_of_the_c_entry(pkg, rows, n, k, kernel, tokens, warps):
+    """b2 without segments: every kernel and tile, all of them ragged; what surrounds the output stays."""
+    dtype = (torch.bfloat16, torch.float16, torch.float32)[(rows + k) % 3]
+    a, sa = T._codes(rows, k, rows), T._scale(rows, 2, 0.01)
+    w, sw = [T._codes(n, k, 3 + i) for i in range(2)], [T._scale(n, 5 + i, 0.002) for i in range(2)]
+    big = torch.full((rows + 2, n + 3), 7.0, dtype=dtype, device="cuda")
+    out = big[1:rows + 1, 1:n + 1]
+    N = pkg._native
+    p = N.Int8Product(a=a.data_ptr(), b=w[0].data_ptr(), b2=w[1].data_ptr(), a_scale=sa.data_ptr(),
+                      b_scale=sw[0].data_ptr(), b2_scale=sw[1].data_ptr(), out=out.data_ptr(), rows=rows,
+                      lda=a.stride(0), ldb=w[0].stride(0), ldo=big.stride(0), n=n, k=k, num_experts=1,
+                      out_dtype=[torch.bfloat16, torch.float16, torch.float32].index(dtype))
+    lib = pkg.load_library()
+    N.check(lib.nvfp4_int8_gemm(ctypes.byref(p), torch.cuda.current_stream().cuda_stream), lib)
+    assert pkg.check_int8_errors() == 0
+    g, up = (T.O.product(T._np(a), T._np(sa), T._np(b), T._np(s)) for b, s in zip(w, sw))
+    want = T.O.silu(g) * up
+    tol = (16 + 5.4 * np.abs(g)) * T.U * np.abs(want) + 1e-30 * np.abs(up)
+    T._close(out, want, 1.01 * (tol + T.HALF[dtype] * np.abs(want)) + T.TINY[dtype])
+    out.fill_(7.0)
+    assert bool((big == 7).all())

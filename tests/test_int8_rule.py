@@ -33,6 +33,11 @@ def test_short_gated_sums_stay_on_single_ctas(pkg):
         assert C.plan(pkg, rows, 3402, k, len(C.RAGGED), False, sum(C.RAGGED), True)[0] == C.PAIRS
 
 
+@pytest.mark.parametrize("rows,n,k,kernel,tokens,warps", C.DENSE_GATED)
+def test_dense_gated_products(pkg, rows, n, k, kernel, tokens, warps):
+    assert C.plan(pkg, rows, n, k, gated=True) == (kernel, tokens, warps)
+
+
 def test_dense_products(pkg):
     assert C.plan(pkg, 1, 4096, 7168) == (C.BYTES, 1, 2)
     assert C.plan(pkg, 83, 4099, 2011) == (C.TILES, 32, 4)
