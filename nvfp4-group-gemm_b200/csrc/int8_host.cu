@@ -183,8 +183,10 @@ int launch_int8_gemv_split(const nvfp4_int8_product* g, const Int8GemmParams& p,
   constexpr int R = int8_gemv_channels(TB, GATED);
   if (warps == 8) return launch_int8_gemv<TB, R, 8, GATED>(g, p, num_sms, s);
   if (warps == 4) return launch_int8_gemv<TB, R, 4, GATED>(g, p, num_sms, s);
-  if (warps == 2) return launch_int8_gemv<TB, R, 2, GATED>(g, p, num_sms, s);
-  return launch_int8_gemv<TB, R, 1, GATED>(g, p, num_sms, s);
+  // Eight tokens are taken where tiles are fewer than a ninth of the SMs and K is 2048 or more: two
+  // warps always fit.
+  if (TB == 8 || warps == 2) return launch_int8_gemv<TB, R, 2, GATED>(g, p, num_sms, s);
+  if constexpr (TB < 8) return launch_int8_gemv<TB, R, 1, GATED>(g, p, num_sms, s);
 }
 
 template <bool GATED, int WARPS>

@@ -77,3 +77,19 @@ def test_tile_numbers_stay_below_2_to_31_with_a_stride_added(pkg):
     with pytest.raises(pkg.Nvfp4Error, match="too many tiles"):
         C.launch(pkg, rows, n, 16)
     assert C.launch(pkg, rows, n // 2, 16).kernel == C.PAIRS
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_byte_products_of_eight_rows_always_share_k(pkg, gated):
+    """No kernel of eight tokens and one warp per channel exists: the rule never asks for it."""
+    seen = set()
+    for sms in (8, 80, 132, 148, 160):
+        for experts in (1, 2, 3, 5, 8, 16):
+            for n in (1, 127, 128, 129, 300, 410, 1000, 2048, 2100):
+                for k in (1024, 2047, 2048, 4096, 8192, 20000):
+                    for per in (3, 4, 5, 8):
+                        kernel, tokens, warps = C.plan(pkg, 2 * per * experts, n, k, experts, gated, per * experts,
+                                                       True, sms=sms, pairs=max(sms // 2, 1))
+                        if kernel == C.BYTES and tokens == 8:
+                            seen.add(warps)
+    assert seen == {2, 4, 8}
