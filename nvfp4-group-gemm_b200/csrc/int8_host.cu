@@ -241,11 +241,14 @@ int int8_pair_rows(const nvfp4_int8_product* g, bool gated, int ktiles, int clus
 // the smallest token tile that still runs in one wave is taken. Dense, N 4096, K 7168: 256 rows
 // 13.2 with tiles of 64, 16.5 with 128; 512 rows 16.9 with 128, 21.4 with 64.
 //
-// With at most 8 rows per expert and few tiles the weights are streamed by all SMs without
+// With at most 8 rows at once and few tiles the weights are streamed by all SMs without
 // tiles (int8_gemv_kernel.cuh), against these tiles: one row 7.4 and 11.6 us (N 4096, K 7168),
 // 13.7 and 15.6 (N 18432, K 4096); two rows 7.6 and 11.6, 14.1 and 15.4; four rows 10.2 and
 // 11.5, 6.6 and 7.0 (N 7168, K 2048), but 17.5 and 15.5 (N 18432); eight rows 6.4 and 12.1 (N
-// 1024, K 8192), 3.8 and 5.9 (N 2048, K 2048), but 16 and 11.5 (N 4096, K 7168).
+// 1024, K 8192), 3.8 and 5.9 (N 2048, K 2048), but 16 and 11.5 (N 4096, K 7168). Of several experts
+// with a row each on average (64 experts, N 128, K 4096, in passes of one and of two rows, and in
+// tiles of 16): one token's 8 pairs 4.5, 4.5 and 9.6; 32 pairs, skewed, 8.1, 6.4 and 9.8; 64 pairs,
+// even, 9.9, 8.5 and 10.1, skewed 16.7, 12.6 and 9.9 (gated, N 256: 33.7, 26.3 and 16.3).
 //
 // Many tiles: bound by the weights' bytes while an expert's rows fit one tile, so tiles are
 // chosen to hold them with a quarter to spare (64 experts of 64 +- 8 rows, N 4096, K 1536:
@@ -274,8 +277,13 @@ Int8Plan plan_int8(const nvfp4_int8_product* g, int num_sms, int clusters) {
     while (warps > 1 && (groups * warps > num_sms * 32 || g->k < 1024 * warps)) warps /= 2;
     return Int8Plan{NVFP4_INT8_BYTES, tokens, warps, 0};
   };
-  // Experts' counts vary: twice the average, unless each is expected to have one row.
-  const int64_t at_once = g->num_experts > 1 && rows > 1 ? 2 * rows : rows;
+  // Experts' counts vary: twice the average. An average of one is one row each for a single token
+  // (up to eight experts) only; more pairs crowd into popular experts, whose weights would be read
+  // once per row.
+  const int64_t at_once = g->num_experts == 1 ? rows
+                          : rows > 1          ? 2 * rows
+                          : expected <= 8     ? 1
+                          : expected <= 32    ? 2 : 16;
   if (at_once == 1 && tiles < num_sms) return bytes(1);
   if (at_once == 2 && tiles < num_sms) return bytes(2);
   if (at_once <= 4 && (gated ? 4 : 2) * tiles < num_sms && g->k >= 1024) return bytes(4);

@@ -23,6 +23,10 @@ EIGHT_ROWS = [(False, 2048, 2), (False, 4111, 4), (False, 8200, 8), (True, 2100,
 ONE_EXPERT_N = 410
 ONE_EXPERT = [(1, 1000, 1), (1, 2100, 2), (2, 1030, 1), (2, 4111, 4), (4, 1030, 1), (4, 8200, 8)]
 
+# At most one expected row per expert, of 64: (expected rows, kernel, tokens).
+ONE_ROW_N = 250
+ONE_ROW_EACH = [(1, BYTES, 1), (8, BYTES, 1), (9, BYTES, 2), (32, BYTES, 2), (33, TILES, 16), (64, TILES, 16)]
+
 # Gated products of one weight pair without segments (the C entry): (rows, n, k, kernel, tokens, warps).
 DENSE_GATED = [(1, 410, 1000, BYTES, 1, 1), (2, 410, 2100, BYTES, 2, 2), (4, 410, 1030, BYTES, 4, 1),
                (7, 410, 4111, BYTES, 8, 4), (7, 2050, 300, TILES, 16, 4), (60, 5000, 200, TILES, 32, 4),

@@ -107,3 +107,12 @@ def test_dense_gated_products_of_the_c_entry(pkg, rows, n, k, kernel, tokens, wa
     T._close(out, want, 1.01 * (tol + T.HALF[dtype] * np.abs(want)) + T.TINY[dtype])
     out.fill_(7.0)
     assert bool((big == 7).all())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("expected,kernel,tokens", C.ONE_ROW_EACH)
+def test_one_expected_row_each_and_all_of_them_in_one_expert(pkg, expected, kernel, tokens, gated):
+    for counts in ([1] * expected + [0] * (64 - expected), [0] * 7 + [expected] + [0] * 56):
+        offs, rows = C.offsets(counts)
+        T._segments_case(pkg, offs, counts, rows, C.ONE_ROW_N, 1100, gated, torch.bfloat16, expected, seed=expected)
+    assert pkg.check_int8_errors() == 0

@@ -93,3 +93,12 @@ def test_byte_products_of_eight_rows_always_share_k(pkg, gated):
                         if kernel == C.BYTES and tokens == 8:
                             seen.add(warps)
     assert seen == {2, 4, 8}
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("expected,kernel,tokens", C.ONE_ROW_EACH)
+def test_one_expected_row_each_is_certain_for_one_token_only(pkg, expected, kernel, tokens, gated):
+    """As many pairs as experts average one row, but a popular expert has several: the weights must not be
+    read once for each of them."""
+    got = C.plan(pkg, 64 * 128, C.ONE_ROW_N, 1100, 64, gated, expected, True)
+    assert got[:2] == (kernel, tokens)
