@@ -11,7 +11,8 @@
 // with tokens as the 256-row operand a ragged expert computed up to 255 rows of padding (64
 // experts of 128 +- 11 rows, gated, N 1536, K 4096: 168 us against 149; of 64 +- 8 rows, N 4096,
 // K 1536: 84 against 71). 8192 x 4096 x 7168 takes 151 us (3.2 POP/s, 0.97 of twice the measured
-// bf16 rate), 182 us in seconds-long runs under the power cap (0.96 of that rate there).
+// bf16 rate), and 182 to 197 us from one GPU to the next in seconds-long runs under the power cap
+// (0.89 to 0.96 of that rate there).
 //
 // Gated: a CTA's 128 rows are 64 of each weight set, so a channel's gate and up sums are 64
 // lanes apart, in two epilogue warps. Per 16 tokens each of the two hands the other its scaled

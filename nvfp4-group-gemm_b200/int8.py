@@ -200,8 +200,9 @@ def int8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: 
     """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k] (+ bias[n])``.
 
     ``a`` int8 [M, K] (codes of tokens), ``b`` int8 [N, K] (codes of weight rows), scales fp32
-    [M] and [N], ``bias`` fp32 [N]. The sums are exact; the result is rounded once, to
-    ``out_dtype`` (bf16 by default; fp16, fp32). Any M, N and K up to 131071; ``out`` may have
+    [M] and [N], ``bias`` fp32 [N]. The sums are exact; they are multiplied with ``a_scale``, then
+    with ``b_scale`` in fp32 (a product past its range is an infinity), and the result is rounded
+    once, to ``out_dtype`` (bf16 by default; fp16, fp32). Any M, N and K up to 131071; ``out`` may have
     any row stride and alignment. ``error_word``: where a wait that timed out is reported (see
     :func:`check_int8_errors`).
     """
@@ -252,7 +253,8 @@ def int8_gemm_segments(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     ``a`` int8 [R, K] with scales [R]; expert e multiplies rows ``[seg_offsets[e],
     seg_offsets[e] + seg_counts[e])`` by its weights ``b[e]`` (int8 [E, N, K], scales [E, N])
     into the same rows of ``out`` [R, N]. With ``b2`` / ``b2_scale`` (same shapes) the result is
-    ``silu(product with b) * (product with b2)``, fp32 until its one rounding. ``seg_offsets``
+    ``silu(product with b) * (product with b2)``, fp32 until its one rounding (with the fast
+    exponential and division where that is to 16 bits). ``seg_offsets``
     and ``seg_counts`` are int32 CUDA tensors (a routing's offsets and counts): nothing is read
     back, so the call can be captured in a CUDA graph. Segments may start anywhere; rows outside
     all of them are left as they were (undefined where ``out`` is allocated here). A segment

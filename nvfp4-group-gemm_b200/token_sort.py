@@ -6,7 +6,8 @@
     out = combine_tokens(rows, r, topk_weights)  # [tokens, H]
 
 bf16, fp16 and fp32, any width and row stride, differentiable in ``x``, the rows and the
-weights (with weights: once). Sums are fp32 in slot order, rounded once: results do not depend on
+weights (with weights: once). Weights of any floating-point type are converted to fp32 first
+(fp64 ones lose bits by that). Sums are fp32 in slot order, rounded once: results do not depend on
 timing.
 The ``*_backward`` functions are the gradients by themselves, for training loops that do not go
 through autograd.
@@ -236,7 +237,7 @@ def combine_tokens(y: torch.Tensor, routing, weights: torch.Tensor | None = None
                    stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """``out[t] = sum_j weights[t, j] * y[routing.dest[t, j]]`` (``weights`` None: ones), ``y``
     bf16, fp16 or fp32 ``[routing.rows, H]``, the result in its type; dropped pairs add nothing.
-    Products and sums are fp32. Differentiable in ``y`` and ``weights``. (:func:`moe.combine` is
+    Weights are taken in fp32 whatever their type, products and sums are fp32. Differentiable in ``y`` and ``weights``. (:func:`moe.combine` is
     the inference form from fp16 rows to bf16.)"""
     if stream is None:
         return _CombineTokens.apply(y, weights, routing)
