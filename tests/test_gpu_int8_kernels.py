@@ -116,3 +116,14 @@ def test_one_expected_row_each_and_all_of_them_in_one_expert(pkg, expected, kern
         offs, rows = C.offsets(counts)
         T._segments_case(pkg, offs, counts, rows, C.ONE_ROW_N, 1100, gated, torch.bfloat16, expected, seed=expected)
     assert pkg.check_int8_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k,kernel", [(100, 200, 1, C.TILES), (40, 3000, 15, C.TILES), (600, 10000, 3, C.PAIRS),
+                                          (300, 20000, 16, C.PAIRS)])
+def test_sums_shorter_than_a_load(pkg, m, n, k, kernel, dtype):
+    assert C.plan(pkg, m, n, k)[0] == kernel
+    a, b = T._codes(m, k, 1), T._codes(n, k, 2)
+    sa, sb = T._scale(m, 3, 0.01), T._scale(n, 4, 0.01)
+    T._check_product(pkg.int8_gemm(a, sa, b, sb, out_dtype=dtype), a, sa, b, sb)
+    assert pkg.check_int8_errors() == 0
